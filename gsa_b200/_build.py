@@ -13,9 +13,12 @@ so that the per-query-walk and exact full-scan fallbacks are exercised, and
 ``gsa_bvh_cap8.so`` caps every tree's stored nodes at 8 so that the
 node-capacity overflow path (exact scans) is exercised; ``gsa_fps_drop.so``
 (FPS only) has one grid block that never arrives at the FPS grid barrier,
-so the barrier's bounded wait runs out and reports its error flag.  Flags keep GSA's arithmetic contract (``scripts/build.py:25-34``:
+so the barrier's bounded wait runs out and reports its error flag;
+``point_features.so`` holds the operators on the points' features (rotary
+positions, cross attention, attention along neighbour rows).  Flags keep GSA's arithmetic contract (``scripts/build.py:25-34``:
 ``--fmad=false --ftz=false``); the kernels also use explicit round-to-nearest
-intrinsics for every distance operation.
+intrinsics for every distance operation (``point_features`` is outside that
+contract and lets the compiler fuse).
 """
 
 import os
@@ -30,10 +33,9 @@ CSRC = PKG / "csrc"
 NATIVE = PKG / "_native"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
+EXACT = ["--fmad=false", "--ftz=false"]  # GSA's arithmetic contract
 FLAGS = [
     "-O3",
-    "--fmad=false",
-    "--ftz=false",
     "-std=c++17",
     "-lineinfo",
     "-Xcompiler",
@@ -62,6 +64,11 @@ LIBS = {
     "gsa_fps_drop": (["launches.cu", "fps.cu"],
                      ["-DGSA_FPS_DROP_BLOCK=1", "-DGSA_FPS_BARRIER_SPINS=65536"]),
 }
+# Operators on the points' features: no part of GSA's contract, free to fuse
+# multiplications with additions.
+_FUSED_ARITHMETIC = {"point_features"}
+LIBS["point_features"] = (
+    ["launches.cu", "rotary.cu", "neighbors.cu", "cross_forward.cu", "cross_backward.cu"], ["-t5"])
 
 
 def nvcc():
@@ -92,7 +99,8 @@ def build(names=None, force=False, verbose=False, extra=()):
         if not force and not _stale(out, sources):
             continue
         tmp = out.with_suffix(".so.tmp%d" % os.getpid())
-        cmd = [nvcc()] + ARCH + FLAGS + list(defs) + list(extra) + [str(s) for s in sources] + ["-o", str(tmp)]
+        exact = [] if name in _FUSED_ARITHMETIC else EXACT
+        cmd = [nvcc()] + ARCH + FLAGS + exact + list(defs) + list(extra) + [str(s) for s in sources] + ["-o", str(tmp)]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)

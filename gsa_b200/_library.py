@@ -57,9 +57,12 @@ def stream():
 
 def launch_counter():
     """Kernel launches the native libraries have enqueued in this process
-    (both libraries' counters added; a replayed CUDA graph adds nothing)."""
+    (the libraries' counters added; a replayed CUDA graph adds nothing)."""
     total = 0
-    for name in ("gsa_bvh", "reference_queries"):
+    names = ["gsa_bvh", "reference_queries"]
+    if "point_features" in _loaded:  # counts nothing before its first use
+        names.append("point_features")
+    for name in names:
         lib = load(name)
         v = ctypes.c_ulonglong()
         lib.launch_counter.argtypes = [ctypes.POINTER(ctypes.c_ulonglong)]

@@ -1,0 +1,703 @@
+// SPDX-License-Identifier: Apache-2.0
+// Attention along the rows of a neighbour query.  Query row r of scene i,
+// head h, reads the entries j of its row of scene-local key IDs:
+//
+//   s_j = scale <q, k_j>,  p = softmax(s),  out = sum_j p_j v_j,
+//   lse = log sum_j exp s_j,
+//
+// over the entries that name a row of the scene's keys and, in padded rows
+// (the radius query's: ascending IDs, then the first again), do not repeat
+// the first entry.  A row without entries gives 0 and lse = -inf.  Backward,
+// with p_j = exp(s_j - lse) and delta = <dout, out>:
+//
+//   ds_j = p_j (<dout, v_j> - delta),   dq = scale sum_j ds_j k_j,
+//   dv[key] = sum p dout,   dk[key] = scale sum ds q
+//
+// over all (row, entry) that name the key: the entries are sorted by key
+// first (stable), so the sums have one fixed order and need no atomics.
+//
+// The bound is the gather: every entry reads a key's and a value's head
+// through L2, D elements each, some tens of times what the tensors hold.  So
+// a head is a group of lanes with a 16-byte vector each, eight entries' loads
+// are in flight per group, and scores, softmax and sums stay in 32-bit
+// registers.
+#include "features.cuh"
+
+namespace gsa {
+namespace {
+
+struct NeighborArgs {
+  const void *q, *k, *v, *out, *dout;
+  void *o, *dq, *dk, *dv;
+  float *lse_out, *delta;
+  const float* lse;
+  const int* ids;    // [n_q][width], scene-local
+  const int *q_seg, *k_seg;
+  const int* starts;  // [n_k + 1]: a key's entries in `order`
+  const int* order;   // query rows, sorted by the key they name
+  long long n_q, n_k;
+  long long q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, d_row,
+      d_head;
+  int scenes, heads, kv_heads, group, dim, width, padded;
+  float scale, scale_log2e;
+};
+
+constexpr int kBlock = 128;
+constexpr int kAhead = 8;  // entries whose loads are in flight
+
+template <int L>
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
+  return x;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ float dot(const uint4& a, const float* b) {
+  float f[V], s = 0.f;
+  Vec<T>::unpack(a, f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) s = fmaf(f[i], b[i], s);
+  return s;
+}
+
+// The keys that entries j0 .. j0 + kAhead of a row name (global key rows), or
+// -1 where an entry is absent.
+__device__ __forceinline__ void entries(const NeighborArgs& a, const int* ids,
+                                        int j0, int first, int base, int n,
+                                        int* at) {
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) {
+    const int j = j0 + t;
+    int id = j < a.width ? __ldg(ids + j) : -1;
+    if (a.padded && j > 0 && id == first) id = -1;
+    at[t] = (unsigned)id < (unsigned)n ? base + id : -1;
+  }
+}
+
+// One group of L lanes per (row, head).
+template <typename T, int L>
+__global__ void __launch_bounds__(kBlock)
+    neighbor_forward_kernel(const __grid_constant__ NeighborArgs a) {
+  constexpr int V = Vec<T>::V;
+  const long long unit =
+      ((long long)blockIdx.x * kBlock + threadIdx.x) / L;
+  const int j = threadIdx.x % L;
+  const long long total = a.n_q * a.heads;
+  const bool live = unit < total;
+  const long long row = live ? unit / a.heads : 0;
+  const int h = live ? (int)(unit - row * a.heads) : 0;
+  const bool mine = live && j * V < a.dim;
+  float q[V], acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) q[i] = acc[i] = 0.f;
+  if (mine)
+    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
+                       static_cast<const T*>(a.q) + row * a.q_row +
+                       h * a.q_head + j * V), q);
+  const int scene = scene_of(a.q_seg, a.scenes, (int)row);
+  const int base = __ldg(a.k_seg + scene);
+  const int n = live ? __ldg(a.k_seg + scene + 1) - base : 0;
+  const int hk = h / a.group;
+  const T* k = static_cast<const T*>(a.k) + hk * a.k_head + j * V;
+  const T* v = static_cast<const T*>(a.v) + hk * a.v_head + j * V;
+  const int* ids = a.ids + row * a.width;
+  const int first = __ldg(ids);
+  float m = -kInf, l = 0.f;
+  bool any = false;
+  for (int j0 = 0; j0 < a.width; j0 += kAhead) {
+    int at[kAhead];
+    entries(a, ids, j0, first, base, n, at);
+    bool here = false;
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) here |= at[t] >= 0;
+    if (!__any_sync(kFull, here)) continue;
+    any |= here;
+    uint4 ku[kAhead], vu[kAhead];
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      ku[t] = vu[t] = make_uint4(0, 0, 0, 0);
+      if (mine && at[t] >= 0) {
+        ku[t] = __ldg(reinterpret_cast<const uint4*>(k + at[t] * a.k_row));
+        vu[t] = __ldg(reinterpret_cast<const uint4*>(v + at[t] * a.v_row));
+      }
+    }
+    float s[kAhead], top = m;
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      s[t] = group_sum<L>(dot<T, V>(ku[t], q)) * a.scale_log2e;
+      if (at[t] < 0) s[t] = -kInf;
+      top = fmaxf(top, s[t]);
+    }
+    const float shift = top == -kInf ? 0.f : top;
+    const float keep = exp2_fast(m - shift);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] *= keep;
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      if (at[t] < 0) continue;  // a masked score of NaN counts for nothing
+      const float p = exp2_fast(s[t] - shift);
+      l += p;
+      float f[V];
+      Vec<T>::unpack(vu[t], f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(p, f[i], acc[i]);
+    }
+  }
+  if (!live) return;
+  if (mine) {
+    const float r = any ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = any ? acc[i] * r : 0.f;
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * a.o_row +
+                              h * a.o_head + j * V) = Vec<T>::pack(acc);
+  }
+  if (j == 0 && a.lse_out)
+    a.lse_out[unit] = any ? (m + log2f(l)) * kLn2 : -kInf;
+}
+
+// dq, and delta for the keys' pass.
+template <typename T, int L>
+__global__ void __launch_bounds__(kBlock)
+    neighbor_dq_kernel(const __grid_constant__ NeighborArgs a) {
+  constexpr int V = Vec<T>::V;
+  const long long unit =
+      ((long long)blockIdx.x * kBlock + threadIdx.x) / L;
+  const int j = threadIdx.x % L;
+  const long long total = a.n_q * a.heads;
+  const bool live = unit < total;
+  const long long row = live ? unit / a.heads : 0;
+  const int h = live ? (int)(unit - row * a.heads) : 0;
+  const bool mine = live && j * V < a.dim;
+  float q[V], d[V], acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) q[i] = d[i] = acc[i] = 0.f;
+  float part = 0.f;
+  if (mine) {
+    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
+                       static_cast<const T*>(a.q) + row * a.q_row +
+                       h * a.q_head + j * V), q);
+    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
+                       static_cast<const T*>(a.dout) + row * a.d_row +
+                       h * a.d_head + j * V), d);
+    part = dot<T, V>(*reinterpret_cast<const uint4*>(
+                         static_cast<const T*>(a.out) + row * a.o_row +
+                         h * a.o_head + j * V), d);
+  }
+  const float delta = group_sum<L>(part);
+  if (live && j == 0) a.delta[unit] = delta;
+  const float lse2 = live ? __ldg(a.lse + unit) * kLog2e : 0.f;
+  const int scene = scene_of(a.q_seg, a.scenes, (int)row);
+  const int base = __ldg(a.k_seg + scene);
+  const int n = live ? __ldg(a.k_seg + scene + 1) - base : 0;
+  const int hk = h / a.group;
+  const T* k = static_cast<const T*>(a.k) + hk * a.k_head + j * V;
+  const T* v = static_cast<const T*>(a.v) + hk * a.v_head + j * V;
+  const int* ids = a.ids + row * a.width;
+  const int first = __ldg(ids);
+  for (int j0 = 0; j0 < a.width; j0 += kAhead) {
+    int at[kAhead];
+    entries(a, ids, j0, first, base, n, at);
+    bool here = false;
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) here |= at[t] >= 0;
+    if (!__any_sync(kFull, here)) continue;
+    uint4 ku[kAhead], vu[kAhead];
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      ku[t] = vu[t] = make_uint4(0, 0, 0, 0);
+      if (mine && at[t] >= 0) {
+        ku[t] = __ldg(reinterpret_cast<const uint4*>(k + at[t] * a.k_row));
+        vu[t] = __ldg(reinterpret_cast<const uint4*>(v + at[t] * a.v_row));
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      float f[V];
+      Vec<T>::unpack(ku[t], f);
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) s = fmaf(f[i], q[i], s);
+      s = group_sum<L>(s);
+      const float dp = group_sum<L>(dot<T, V>(vu[t], d));
+      if (at[t] < 0) continue;
+      const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2));
+      const float ds = p * (dp - delta);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(ds, f[i], acc[i]);
+    }
+  }
+  if (mine) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] *= a.scale;
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.dq) +
+                              unit * a.dim + j * V) = Vec<T>::pack(acc);
+  }
+}
+
+// dk and dv: a warp per (key, head of keys); its 32 / L groups take the key's
+// (entry, query head) pairs in turn and are added up at the end.
+template <typename T, int L>
+__global__ void __launch_bounds__(kBlock)
+    neighbor_dkv_kernel(const __grid_constant__ NeighborArgs a) {
+  constexpr int V = Vec<T>::V;
+  constexpr int G = 32 / L;
+  constexpr int kDeep = 4;
+  const long long unit =
+      ((long long)blockIdx.x * kBlock + threadIdx.x) >> 5;
+  if (unit >= a.n_k * a.kv_heads) return;  // the whole warp
+  const int lane = threadIdx.x & 31, j = lane % L, who = lane / L;
+  const long long key = unit / a.kv_heads;
+  const int hk = (int)(unit - key * a.kv_heads);
+  const bool mine = j * V < a.dim;
+  float k[V], v[V], dk[V], dv[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) k[i] = v[i] = dk[i] = dv[i] = 0.f;
+  if (mine) {
+    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
+                       static_cast<const T*>(a.k) + key * a.k_row +
+                       hk * a.k_head + j * V), k);
+    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
+                       static_cast<const T*>(a.v) + key * a.v_row +
+                       hk * a.v_head + j * V), v);
+  }
+  const int from = __ldg(a.starts + key);
+  const long long pairs =
+      (long long)(__ldg(a.starts + key + 1) - from) * a.group;
+  for (long long t0 = 0; t0 < pairs; t0 += G * kDeep) {
+    uint4 qu[kDeep], du[kDeep];
+    float lse2[kDeep], delta[kDeep];
+#pragma unroll
+    for (int t = 0; t < kDeep; ++t) {
+      const long long at = t0 + t * G + who;
+      qu[t] = du[t] = make_uint4(0, 0, 0, 0);
+      lse2[t] = kInf;  // absent: p = 0
+      delta[t] = 0.f;
+      if (at < pairs) {
+        const long long e = at / a.group;
+        const int h = hk * a.group + (int)(at - e * a.group);
+        const long long row = __ldg(a.order + from + e);
+        lse2[t] = __ldg(a.lse + row * a.heads + h) * kLog2e;
+        delta[t] = __ldg(a.delta + row * a.heads + h);
+        if (mine) {
+          qu[t] = __ldg(reinterpret_cast<const uint4*>(
+              static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head +
+              j * V));
+          du[t] = __ldg(reinterpret_cast<const uint4*>(
+              static_cast<const T*>(a.dout) + row * a.d_row + h * a.d_head +
+              j * V));
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kDeep; ++t) {
+      float f[V], g[V], s = 0.f, dp = 0.f;
+      Vec<T>::unpack(qu[t], f);
+      Vec<T>::unpack(du[t], g);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        s = fmaf(f[i], k[i], s);
+        dp = fmaf(g[i], v[i], dp);
+      }
+      s = group_sum<L>(s);
+      dp = group_sum<L>(dp);
+      if (t0 + t * G + who >= pairs) continue;
+      const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2[t]));
+      const float ds = p * (dp - delta[t]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        dk[i] = fmaf(ds, f[i], dk[i]);
+        dv[i] = fmaf(p, g[i], dv[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int o = L; o < 32; o <<= 1) {
+      dk[i] += __shfl_xor_sync(kFull, dk[i], o);
+      dv[i] += __shfl_xor_sync(kFull, dv[i], o);
+    }
+    dk[i] *= a.scale;
+  }
+  if (who == 0 && mine) {
+    const long long at = unit * a.dim + j * V;
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.dk) + at) = Vec<T>::pack(dk);
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.dv) + at) = Vec<T>::pack(dv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Entries sorted by key: a stable radix sort of (key, query row), absent
+// entries last under the key n_k.  Per digit: counts per tile, their prefix
+// per digit value, scatter.  Ranks inside a tile follow the entries' order.
+
+constexpr int kSortThreads = 256;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortEach = 8;                     // entries per thread
+constexpr int kTile = kSortThreads * kSortEach;  // entries per tile
+constexpr int kMaxDigitBits = 9;
+constexpr int kMaxBins = 1 << kMaxDigitBits;
+
+struct SortArgs {
+  const unsigned* keys_in;
+  const int* rows_in;
+  unsigned* keys_out;
+  int* rows_out;
+  int* counts;  // [bins][tiles], then [bins] totals
+  long long n;
+  int tiles, shift, bits;
+};
+
+// keys[e]: the key row that entry e names, or n_k; rows[e]: its query row.
+__global__ void __launch_bounds__(256)
+    entry_keys_kernel(const __grid_constant__ NeighborArgs a, unsigned* keys,
+                      int* rows) {
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= a.n_q * a.width) return;
+  const long long row = e / a.width;
+  const int scene = scene_of(a.q_seg, a.scenes, (int)row);
+  const int base = __ldg(a.k_seg + scene);
+  const int n = __ldg(a.k_seg + scene + 1) - base;
+  int id = __ldg(a.ids + e);
+  if (a.padded && e != row * a.width && id == __ldg(a.ids + row * a.width))
+    id = -1;
+  keys[e] = (unsigned)id < (unsigned)n ? (unsigned)(base + id)
+                                       : (unsigned)a.n_k;
+  rows[e] = (int)row;
+}
+
+__global__ void __launch_bounds__(kSortThreads)
+    sort_count_kernel(const __grid_constant__ SortArgs a) {
+  __shared__ int bins[kMaxBins];
+  const int n_bins = 1 << a.bits;
+  for (int i = threadIdx.x; i < n_bins; i += kSortThreads) bins[i] = 0;
+  __syncthreads();
+  const long long at = (long long)blockIdx.x * kTile;
+#pragma unroll
+  for (int t = 0; t < kSortEach; ++t) {
+    const long long e = at + t * kSortThreads + threadIdx.x;
+    if (e < a.n)
+      atomicAdd(&bins[(a.keys_in[e] >> a.shift) & (n_bins - 1)], 1);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_bins; i += kSortThreads)
+    a.counts[(long long)i * a.tiles + blockIdx.x] = bins[i];
+}
+
+// Inclusive sum over the block's kSortThreads values.
+__device__ __forceinline__ int block_inclusive(int x, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(kFull, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  return x + before;
+}
+
+// A block per digit value: its tiles' counts become their exclusive prefix.
+__global__ void __launch_bounds__(kSortThreads)
+    sort_scan_kernel(const __grid_constant__ SortArgs a) {
+  __shared__ int warp_sums[kSortWarps];
+  __shared__ int last;
+  int* row = a.counts + (long long)blockIdx.x * a.tiles;
+  int carry = 0;
+  for (int t0 = 0; t0 < a.tiles; t0 += kSortThreads) {
+    const int t = t0 + threadIdx.x;
+    const int x = t < a.tiles ? row[t] : 0;
+    const int sum = block_inclusive(x, warp_sums);
+    if (t < a.tiles) row[t] = carry + sum - x;
+    if (threadIdx.x == kSortThreads - 1) last = sum;
+    __syncthreads();
+    carry += last;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0)
+    a.counts[(long long)(1 << a.bits) * a.tiles + blockIdx.x] = carry;
+}
+
+__global__ void __launch_bounds__(kSortThreads)
+    sort_scatter_kernel(const __grid_constant__ SortArgs a) {
+  __shared__ int count[kSortWarps][kMaxBins];  // then: where the warp's begin
+  __shared__ int warp_sums[kSortWarps];
+  const int n_bins = 1 << a.bits;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = lane; i < n_bins; i += 32) count[warp][i] = 0;
+  __syncwarp();
+  // a warp's entries are consecutive, 32 at a time in their order
+  const long long at =
+      (long long)blockIdx.x * kTile + warp * (32 * kSortEach);
+  unsigned key[kSortEach];
+  int row[kSortEach], rank[kSortEach];
+#pragma unroll
+  for (int t = 0; t < kSortEach; ++t) {
+    const long long e = at + t * 32 + lane;
+    key[t] = e < a.n ? a.keys_in[e] : 0u;
+    row[t] = e < a.n ? a.rows_in[e] : 0;
+  }
+#pragma unroll
+  for (int t = 0; t < kSortEach; ++t) {
+    const bool live = at + t * 32 + lane < a.n;
+    const unsigned digit = (key[t] >> a.shift) & (n_bins - 1);
+    const unsigned peers =
+        __match_any_sync(kFull, live ? digit : 0xffffffffu);
+    const int before = __popc(peers & ((1u << lane) - 1));
+    rank[t] = live ? count[warp][digit] + before : 0;
+    __syncwarp();
+    if (live && before == 0) count[warp][digit] += __popc(peers);
+    __syncwarp();
+  }
+  __syncthreads();
+  // start of every digit value's run in the output, for this tile
+  int carry = 0;
+  for (int b0 = 0; b0 < n_bins; b0 += kSortThreads) {
+    const int b = b0 + threadIdx.x;
+    const int total =
+        b < n_bins ? a.counts[(long long)n_bins * a.tiles + b] : 0;
+    const int sum = block_inclusive(total, warp_sums);
+    if (b < n_bins) {
+      int begin = carry + sum - total +
+                  a.counts[(long long)b * a.tiles + blockIdx.x];
+      for (int w = 0; w < kSortWarps; ++w) {
+        const int c = count[w][b];
+        count[w][b] = begin;
+        begin += c;
+      }
+    }
+    int all = 0;
+    for (int w = 0; w < kSortWarps; ++w) all += warp_sums[w];
+    carry += all;
+    __syncthreads();
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < kSortEach; ++t) {
+    if (at + t * 32 + lane >= a.n) continue;
+    const int digit = (key[t] >> a.shift) & (n_bins - 1);
+    const int to = count[warp][digit] + rank[t];
+    a.keys_out[to] = key[t];
+    a.rows_out[to] = row[t];
+  }
+}
+
+// starts[key] for every key 0 .. n_k: the first sorted entry not below it.
+__global__ void __launch_bounds__(256)
+    key_starts_kernel(const unsigned* keys, int n, long long n_k,
+                      int* starts) {
+  const long long key = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (key > n_k) return;
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (__ldg(keys + mid) < (unsigned)key) lo = mid + 1; else hi = mid;
+  }
+  starts[key] = lo;
+}
+
+struct SortPlan {
+  int passes, bits, tiles;
+};
+
+SortPlan sort_plan(long long n, long long n_k) {
+  int key_bits = 1;
+  while ((1ll << key_bits) <= n_k) ++key_bits;
+  SortPlan p;
+  p.passes = (key_bits + kMaxDigitBits - 1) / kMaxDigitBits;
+  p.bits = (key_bits + p.passes - 1) / p.passes;
+  p.tiles = (int)ceil_div(n, kTile);
+  return p;
+}
+
+long long align16(long long bytes) { return (bytes + 15) & ~15ll; }
+
+// ---------------------------------------------------------------------------
+
+template <typename T, int L>
+cudaError_t forward(const NeighborArgs& a, cudaStream_t s) {
+  const long long lanes = a.n_q * a.heads * L;
+  count_launches(1);
+  neighbor_forward_kernel<T, L>
+      <<<(unsigned)ceil_div(lanes, kBlock), kBlock, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T, int L>
+cudaError_t backward(const NeighborArgs& a, cudaStream_t s) {
+  if (a.n_q) {
+    const long long lanes = a.n_q * a.heads * L;
+    count_launches(1);
+    neighbor_dq_kernel<T, L>
+        <<<(unsigned)ceil_div(lanes, kBlock), kBlock, 0, s>>>(a);
+  }
+  if (a.n_k) {
+    count_launches(1);
+    neighbor_dkv_kernel<T, L>
+        <<<(unsigned)ceil_div(a.n_k * a.kv_heads, kBlock / 32), kBlock, 0, s>>>(
+            a);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run(const NeighborArgs& a, bool back, cudaStream_t s) {
+  const int vectors = a.dim / Vec<T>::V;
+#define GSA_LANES(L) \
+  if (vectors <= L) return back ? backward<T, L>(a, s) : forward<T, L>(a, s)
+  if constexpr (Vec<T>::V == 8) GSA_LANES(1);
+  GSA_LANES(2);
+  GSA_LANES(4);
+  GSA_LANES(8);
+  GSA_LANES(16);
+  if constexpr (Vec<T>::V == 4) GSA_LANES(32);
+#undef GSA_LANES
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t run_type(const NeighborArgs& a, int type, bool back,
+                     cudaStream_t s) {
+  if (type == kF32) return run<float>(a, back, s);
+  if (type == kF16) return run<__half>(a, back, s);
+  return run<__nv_bfloat16>(a, back, s);
+}
+
+bool sizes_ok(const attention_args* a) {
+  return attention_sizes(a) && a->width >= 1 && a->width <= 32 &&
+         a->n_q * a->width < kMaxInt;
+}
+
+NeighborArgs arguments(const attention_args* in) {
+  NeighborArgs a = {};
+  a.q = in->q.data;
+  a.k = in->k.data;
+  a.v = in->v.data;
+  a.ids = in->ids;
+  a.q_seg = in->q_seg;
+  a.k_seg = in->k_seg;
+  a.scenes = (int)in->scenes;
+  a.n_q = in->n_q;
+  a.n_k = in->n_k;
+  a.q_row = in->q.row;
+  a.q_head = in->q.head;
+  a.k_row = in->k.row;
+  a.k_head = in->k.head;
+  a.v_row = in->v.row;
+  a.v_head = in->v.head;
+  a.o_row = in->out.row;
+  a.o_head = in->out.head;
+  a.heads = (int)in->heads;
+  a.kv_heads = (int)in->kv_heads;
+  a.group = a.heads / a.kv_heads;
+  a.dim = (int)in->dim;
+  a.width = (int)in->width;
+  a.padded = in->padded != 0;
+  a.scale = (float)in->scale;
+  a.scale_log2e = (float)(in->scale * (double)kLog2e);
+  return a;
+}
+
+}  // namespace
+}  // namespace gsa
+
+using namespace gsa;
+
+// See include/point_features.h.
+GSA_API int neighbor_attention(const attention_args* in) {
+  if (!sizes_ok(in) || !attention_scale(in->scale)) return -2;
+  if (!in->n_q) return 0;
+  if (!vector_rows(in->q, in->type) || !vector_rows(in->out, in->type) ||
+      !in->ids || !in->q_seg || !in->k_seg)
+    return -2;
+  if (in->n_k &&
+      (!vector_rows(in->k, in->type) || !vector_rows(in->v, in->type)))
+    return -2;
+  NeighborArgs a = arguments(in);
+  a.o = const_cast<void*>(in->out.data);
+  a.lse_out = in->lse;
+  return run_type(a, (int)in->type, false, (cudaStream_t)in->stream);
+}
+
+// See include/point_features.h.
+GSA_API int64_t neighbor_attention_grad_workspace(const attention_args* in) {
+  if (!sizes_ok(in)) return -2;
+  const long long n = in->n_q * in->width;
+  const SortPlan p = sort_plan(n, in->n_k);
+  return align16(in->n_q * in->heads * 4) + 4 * align16(n * 4) +
+         align16((in->n_k + 1) * 4) +
+         align16((1ll << p.bits) * (p.tiles + 1) * 4);
+}
+
+// See include/point_features.h.
+GSA_API int neighbor_attention_grad(const attention_args* in) {
+  if (!sizes_ok(in) || !attention_scale(in->scale) || !in->q_seg ||
+      !in->k_seg)
+    return -2;
+  const long long type = in->type, n_q = in->n_q, n_k = in->n_k;
+  if (n_q && (!vector_rows(in->q, type) || !vector_rows(in->out, type) ||
+              !vector_rows(in->dout, type) || !vector_address(in->dq) ||
+              !in->lse || !in->ids))
+    return -2;
+  if (n_k && (!vector_rows(in->k, type) || !vector_rows(in->v, type) ||
+              !vector_address(in->dk) || !vector_address(in->dv)))
+    return -2;
+  if (!vector_address(in->workspace) ||
+      in->workspace_bytes < neighbor_attention_grad_workspace(in))
+    return -2;
+  NeighborArgs a = arguments(in);
+  a.out = in->out.data;
+  a.dout = in->dout.data;
+  a.d_row = in->dout.row;
+  a.d_head = in->dout.head;
+  a.lse = in->lse;
+  a.dq = in->dq;
+  a.dk = in->dk;
+  a.dv = in->dv;
+  cudaStream_t s = (cudaStream_t)in->stream;
+  const long long n = n_q * a.width;
+  const SortPlan p = sort_plan(n, n_k);
+  char* at = static_cast<char*>(in->workspace);
+  auto take = [&](long long bytes) {
+    char* r = at;
+    at += align16(bytes);
+    return r;
+  };
+  a.delta = reinterpret_cast<float*>(take(n_q * a.heads * 4));
+  unsigned* keys[2];
+  int* rows[2];
+  for (int i = 0; i < 2; ++i) {
+    keys[i] = reinterpret_cast<unsigned*>(take(n * 4));
+    rows[i] = reinterpret_cast<int*>(take(n * 4));
+  }
+  int* starts = reinterpret_cast<int*>(take((n_k + 1) * 4));
+  int* counts =
+      reinterpret_cast<int*>(take((1ll << p.bits) * (p.tiles + 1) * 4));
+  int from = 0;
+  if (n && n_k) {
+    count_launches(1 + 3 * p.passes);
+    entry_keys_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(a, keys[0],
+                                                                 rows[0]);
+    for (int pass = 0; pass < p.passes; ++pass, from ^= 1) {
+      SortArgs t = {keys[from],     rows[from], keys[from ^ 1],
+                    rows[from ^ 1], counts,     n,
+                    p.tiles,        pass * p.bits, p.bits};
+      sort_count_kernel<<<p.tiles, kSortThreads, 0, s>>>(t);
+      sort_scan_kernel<<<1 << p.bits, kSortThreads, 0, s>>>(t);
+      sort_scatter_kernel<<<p.tiles, kSortThreads, 0, s>>>(t);
+    }
+  }
+  if (n_k) {
+    count_launches(1);
+    key_starts_kernel<<<(unsigned)ceil_div(n_k + 1, 256), 256, 0, s>>>(
+        keys[from], (int)n, n_k, starts);
+  }
+  a.starts = starts;
+  a.order = rows[from];
+  return run_type(a, (int)type, true, s);
+}

@@ -1,0 +1,135 @@
+# SPDX-License-Identifier: Apache-2.0
+"""Rotary positions of points' features.
+
+``Rotary`` turns the first ``part`` elements of every head by angles that grow
+with the point's position, so that the products of two turned heads depend on
+the difference of their positions only.  Positions are the points' own
+coordinates (``axes`` = 2 or 3: an equal share of the pairs for each) or a
+place in an order (``axes`` = 1), where ``scaling`` extends a network to
+longer orders than it was trained on.
+"""
+
+import ctypes
+import math
+
+import torch
+
+from . import _features as ft
+from ._library import current_stream
+
+MAX_PAIRS = 128  # per axis
+MAX_DIM = 4096
+
+
+def frequencies(pairs, base=10000.0, scaling=None, factor=1.0, length=None, low=1.0, high=32.0):
+    """Radians per unit of position of an axis' pairs: ``base ** (-i / pairs)``,
+    scaled for positions ``factor`` times as far as those trained on.
+
+    ``None``      as they are;
+    ``"linear"``  all divided by ``factor``;
+    ``"base"``    the base grown so that the slowest pair is divided by
+                  ``factor`` and the fastest kept;
+    ``"ramp"``    by how often a pair turns over the ``length`` trained on:
+                  kept from ``high`` turns on, divided up to ``low``, and
+                  blended linearly between."""
+    if scaling == "base" and pairs > 1:
+        base = base * factor ** (pairs / (pairs - 1))
+    f = [base ** (-i / pairs) for i in range(pairs)]
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    elif scaling == "ramp":
+        keep = [min(1.0, max(0.0, (length * x / (2 * math.pi) - low) / (high - low))) for x in f]
+        f = [x * k + x / factor * (1 - k) for x, k in zip(f, keep)]
+    return f
+
+
+class Rotary:
+    """A rotation plan: ``rotary(x, positions)`` returns the turned rows and
+    ``rotary.grad(dy, positions)`` the gradient of ``x``.
+
+    ``part``: elements of a head that turn, a multiple of ``2 * axes``; the
+    others are copied.  ``layout``: ``"half"`` pairs element p with
+    p + part / 2, ``"interleaved"`` 2p with 2p + 1; the pairs of an axis
+    follow one another.  ``unit``: the length that counts as one position.
+    ``base``, ``scaling``, ``factor``, ``length``: see ``frequencies``.
+    ``amplitude``: factor of the turned elements, by default 1, for "ramp"
+    0.1 ln(factor) + 1."""
+
+    def __init__(self, part, axes=1, layout="half", base=10000.0, unit=1.0, scaling=None, factor=1.0, length=None,
+                 amplitude=None):
+        if not (isinstance(part, int) and isinstance(axes, int) and axes >= 1 and part >= 2 and part % (2 * axes) == 0
+                and part // (2 * axes) <= MAX_PAIRS):
+            raise ValueError("part must be a positive multiple of 2 * axes with at most 128 pairs per axis")
+        if layout not in ("half", "interleaved"):
+            raise ValueError("layout is 'half' or 'interleaved'")
+        if scaling not in (None, "linear", "base", "ramp"):
+            raise ValueError("scaling is None, 'linear', 'base' or 'ramp'")
+        if not all(math.isfinite(v) and v > 0 for v in (base, unit, factor)):
+            raise ValueError("base, unit and factor must be positive")
+        if scaling == "ramp" and not (length is not None and math.isfinite(length) and length > 0):
+            raise ValueError("scaling 'ramp' needs the length trained on")
+        if amplitude is None:
+            amplitude = 0.1 * math.log(factor) + 1.0 if scaling == "ramp" else 1.0
+        if not math.isfinite(amplitude):
+            raise ValueError("amplitude must be finite")
+        self.part, self.axes, self.layout, self.amplitude = part, axes, layout, amplitude
+        self.pairs = part // (2 * axes)
+        f = frequencies(self.pairs, base, scaling, factor, length)
+        self._turns = (ctypes.c_double * self.pairs)(*[v / (2 * math.pi) / unit for v in f])
+        self._turns_at = ctypes.addressof(self._turns)
+
+    def _run(self, x, positions, out, transposed):
+        if not (isinstance(x, torch.Tensor) and x.is_cuda and x.ndim == 3 and x.dtype in ft.TYPES and x.shape[1] > 0
+                and self.part <= x.shape[2] <= MAX_DIM):
+            raise ValueError("rows must be CUDA FP32, FP16 or BF16 (N, heads, dim) with dim from part to 4096")
+        device, stream = current_stream()
+        rows, heads, dim = x.shape
+        place = ft.rows_of(x, "rows", x.shape, x.dtype, device)
+        if not (
+            isinstance(positions, torch.Tensor)
+            and positions.is_cuda
+            and positions.get_device() == device
+            and positions.dtype in ft.POSITION_TYPES
+            and (positions.shape == (rows, self.axes) or (self.axes == 1 and positions.shape == (rows,)))
+        ):
+            raise ValueError("positions must be CUDA FP32, int32 or int64 (N, axes) on the rows' device")
+        if out is None:
+            out = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device)
+        to = ft.rows_of(out, "out", x.shape, x.dtype, device)
+        ft.check_written(out, "out")
+        args = ft.pack_rotary(
+            ft.TYPES[x.dtype], rows, heads, dim, *place, *to, positions.data_ptr(), ft.POSITION_TYPES[positions.dtype],
+            positions.stride(0), positions.stride(1) if positions.ndim == 2 else 0, self.axes, self.pairs,
+            self._turns_at, self.amplitude, self.layout == "interleaved", transposed, stream,
+        )
+        ft.check(ft.lib.rotary_positions(args), "rotary positions")
+        return out
+
+    def __call__(self, x, positions, out=None):
+        """The rows ``x`` (FP32, FP16 or BF16 (N, heads, dim), any row and
+        head strides) turned by ``positions`` (FP32, int32 or int64
+        (N, axes), or (N,) for one axis).  ``out`` may be ``x`` itself, else it does not
+        overlap it.  Differentiable in ``x`` when ``out`` is not given."""
+        if out is None and isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+            return _Turn.apply(x, positions, self)
+        return self._run(x, positions, out, False)
+
+    def grad(self, dy, positions, out=None):
+        """The gradient of ``x`` from that of ``rotary(x, positions)``."""
+        return self._run(dy, positions, out, True)
+
+
+class _Turn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, rotary):
+        ctx.save_for_backward(positions)
+        ctx.rotary = rotary
+        return rotary._run(x, positions, None, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (positions,) = ctx.saved_tensors
+        if dy.stride(2) != 1:
+            dy = dy.contiguous()
+        return ctx.rotary._run(dy, positions, None, True), None, None

@@ -1,0 +1,530 @@
+# SPDX-License-Identifier: Apache-2.0
+"""GPU: rotary positions, cross attention and neighbour attention against
+64-bit oracles (``tests/features_oracle.py``, whose bounds are derived there),
+and the ways a program calls them."""
+
+import math
+
+import pytest
+import torch
+
+from tests import features_oracle as fo
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def normal(seed, *shape, dtype=FP32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).cuda()
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+
+
+def check_rotary(x, positions, part, axes, layout, out=None, transposed=False, **plan):
+    from gsa_b200 import Rotary, rotary
+
+    r = Rotary(part, axes=axes, layout=layout, **plan)
+    before = x.clone()
+    got = (r.grad if transposed else r)(x, positions, out=out)
+    f = rotary.frequencies(r.pairs, plan.get("base", 10000.0), plan.get("scaling"), plan.get("factor", 1.0),
+                           plan.get("length"))
+    want, off = fo.rotate(before, positions, f, axes, part, layout, plan.get("unit", 1.0), r.amplitude, transposed)
+    bad = (got.double().cpu() - want).abs() > off
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} elements are too far off"
+    assert torch.equal(got[..., part:], before[..., part:])
+    return got
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows,heads,dim,part,axes", [
+    (1, 1, 8, 8, 1), (5, 3, 16, 16, 1), (33, 8, 32, 30, 3), (257, 5, 48, 36, 3), (19, 2, 64, 32, 1), (7, 9, 128, 128, 2),
+    (3, 4, 40, 2, 1), (70, 1, 256, 256, 1), (6, 2, 20, 18, 3), (5, 3, 7, 6, 1), (2, 2, 300, 256, 1)])
+def test_rotary_shapes(rows, heads, dim, part, axes, dtype, layout):
+    x = normal(1, rows, heads, dim, dtype=dtype)
+    check_rotary(x, normal(2, rows, axes, scale=4.0), part, axes, layout, unit=0.02)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64, FP32])
+@pytest.mark.parametrize("scaling", [None, "linear", "base", "ramp"])
+def test_rotary_far_positions_and_scalings(kind, scaling):
+    x = normal(3, 64, 2, 64, dtype=FP32)
+    g = torch.Generator().manual_seed(4)
+    far = torch.randint(0, 1 << 24, (64,), generator=g)
+    far[0] = 0
+    check_rotary(x, far.to(kind).cuda(), 64, 1, "half", scaling=scaling, factor=16.0, length=4096)
+    check_rotary(x, far.to(kind).cuda(), 64, 1, "interleaved", transposed=True, scaling=scaling, factor=16.0, length=4096)
+
+
+def test_rotary_positions_beyond_32_bits():
+    x = normal(5, 8, 1, 16)
+    far = (torch.arange(8) * 987654321 + (1 << 33)).cuda()
+    check_rotary(x, far, 16, 1, "half")
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,part", [(32, 30), (64, 48), (14, 12)])
+def test_rotary_in_place_strides_and_positions_view(layout, dim, part):
+    x = normal(6, 50, 3, 4, dim, dtype=BF16)
+    place = normal(7, 50, 7)[:, 2:5]
+    separate = check_rotary(x[:, 1], place, part, 3, layout)
+    whole = x.clone()
+    same = whole[:, 1]
+    check_rotary(same, place, part, 3, layout, out=same)
+    assert torch.equal(same, separate)
+    assert torch.equal(whole[:, 0], x[:, 0]) and torch.equal(whole[:, 2], x[:, 2])
+    # heads before rows, in and out; odd addresses
+    t = normal(8, 4, 50, dim, dtype=BF16).transpose(0, 1)
+    out = torch.empty(4, 50, dim, dtype=BF16, device="cuda").transpose(0, 1)
+    check_rotary(t, place, part, 3, layout, out=out)
+    odd = normal(9, 50 * 4 * dim + 1, dtype=BF16)[1:].view(50, 4, dim)
+    check_rotary(odd, place, part, 3, layout)
+
+
+def test_rotary_undoes_itself_and_has_its_gradient():
+    from gsa_b200 import Rotary
+
+    r = Rotary(30, axes=3)
+    x, place = normal(10, 40, 2, 32), normal(11, 40, 3)
+    assert torch.allclose(r.grad(r(x, place), place), x, atol=1e-5)
+    x.requires_grad_()
+    d = normal(12, 40, 2, 32)
+    r(x, place).backward(d)
+    assert torch.equal(x.grad, r.grad(d, place))
+    y = normal(13, 40, 2, 32)  # <turned x, d> = <x, gradient>, by differences
+    h = 2.0**-6
+    moved = [(r(x.detach() + s * h * y, place).double() * d.double()).sum() for s in (1, -1)]
+    # linear in x: only the 32-bit roundings differ, 2^-20 of the sums of |x d| / h
+    bound = 2.0**-20 * ((x.detach().abs() + y.abs()).double() * d.abs().double()).sum() * 2 / h
+    assert (((moved[0] - moved[1]) / (2 * h)) - (x.grad.double() * y.double()).sum()).abs() < bound
+
+
+def test_rotary_refuses():
+    from gsa_b200 import Rotary
+
+    r = Rotary(32, axes=1)
+    x, place = normal(1, 6, 2, 32), torch.arange(6).cuda()
+    assert r(x[:0], place[:0]).shape == (0, 2, 32)
+    for bad in [(x[..., :16], place), (x[..., ::2], place), (x.double(), place), (x[0], place), (x, place[:5]),
+                (x, place.double()), (x, place.cpu()), (x, place[:, None].expand(6, 2)), (x[:, :0], place)]:
+        with pytest.raises(ValueError):
+            r(*bad)
+    for out in (x[:5], x.half(), x.cpu(), x[:, :1].expand(6, 2, 32)):
+        with pytest.raises(ValueError):
+            r(x, place, out=out)
+
+
+# ---------------------------------------------------------------------------
+# attention
+
+
+def lengths_case(name):
+    return {
+        "one": ([1], [1]),
+        "row on many": ([1], [3001]),
+        "few rows on many": ([3, 2], [1500, 900]),
+        "ragged": ([1, 0, 130, 64, 5, 129], [200, 7, 0, 129, 1, 65]),
+        "tiles": ([128, 256], [128, 256]),
+        "many rows": ([700], [70]),
+        "no keys": ([5, 9], [0, 0]),
+        "no queries": ([0, 0], [4, 9]),
+    }[name]
+
+
+def attention_inputs(seed, lengths, heads, kv_heads, dim, dtype, layout="packed", scale=1.0):
+    q_seg, k_seg = fo.seg_of(lengths[0]), fo.seg_of(lengths[1])
+    nq, nk = q_seg[-1], k_seg[-1]
+    if layout == "fused":  # one tensor of keys and values, rows of queries inside wider ones
+        q = normal(seed, nq, heads + 1, dim, dtype=dtype, scale=scale)[:, 1:]
+        kv = normal(seed + 1, nk, 2, kv_heads, dim, dtype=dtype)
+        k, v = kv[:, 0], kv[:, 1]
+    elif layout == "heads first":
+        q = normal(seed, heads, nq, dim, dtype=dtype, scale=scale).transpose(0, 1)
+        k = normal(seed + 1, kv_heads, nk, dim, dtype=dtype).transpose(0, 1)
+        v = normal(seed + 2, kv_heads, nk, dim, dtype=dtype).transpose(0, 1)
+    else:
+        q = normal(seed, nq, heads, dim, dtype=dtype, scale=scale)
+        k, v = normal(seed + 1, nk, kv_heads, dim, dtype=dtype), normal(seed + 2, nk, kv_heads, dim, dtype=dtype)
+    return q, k, v, q_seg, k_seg
+
+
+def check_cross(q, k, v, q_seg, k_seg, mask=None, scale=None, grads=True, seed=77):
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    pairs = ScenePairs(q_seg, k_seg)
+    out, lse = cross_attention(q, k, v, pairs, mask=mask, scale=scale, return_lse=True)
+    dout = normal(seed, *q.shape, dtype=q.dtype) if grads else None
+    want = fo.Attention(q, k, v, q_seg, k_seg, mask=mask, scale=scale, dout=dout)
+    want.close("out", out)
+    want.close("lse", lse)
+    if grads:
+        got = cross_attention_grad(dout, q, k, v, out, lse, pairs, mask=mask, scale=scale)
+        for name, t in zip(("dq", "dk", "dv"), got):
+            want.close(name, t)
+    pairs.check()
+    return want
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("dim", [8, 24, 32, 64, 72, 128])
+@pytest.mark.parametrize("name", ["one", "row on many", "few rows on many", "ragged", "tiles", "many rows"])
+def test_cross_sizes(name, dim, dtype):
+    check_cross(*attention_inputs(20, lengths_case(name), 2, 2, dim, dtype))
+
+
+@pytest.mark.parametrize("dim", [16, 96])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 2), (6, 1), (3, 3), (10, 2)])
+@pytest.mark.parametrize("layout", ["packed", "fused", "heads first"])
+def test_cross_heads_and_layouts(layout, heads, kv_heads, dim):
+    check_cross(*attention_inputs(30, lengths_case("ragged"), heads, kv_heads, dim, BF16, layout))
+
+
+@pytest.mark.parametrize("dim", [32, 128])
+@pytest.mark.parametrize("name", ["no keys", "no queries"])
+def test_cross_empty_sides(name, dim):
+    from gsa_b200 import ScenePairs, cross_attention
+
+    q, k, v, q_seg, k_seg = attention_inputs(40, lengths_case(name), 4, 2, dim, BF16)
+    check_cross(q, k, v, q_seg, k_seg)
+    out, lse = cross_attention(q, k, v, ScenePairs(q_seg, k_seg), return_lse=True)
+    assert not out.any() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (48, FP16), (128, BF16)])
+@pytest.mark.parametrize("name", ["ragged", "few rows on many", "tiles"])
+def test_cross_masked_keys_may_hold_anything(name, dim, dtype):
+    q, k, v, q_seg, k_seg = attention_inputs(50, lengths_case(name), 4, 2, dim, dtype)
+    g = torch.Generator().manual_seed(51)
+    mask = torch.rand(len(k), generator=g) < 0.6
+    mask[k_seg[-2]:] = False  # a whole scene shut
+    mask[k_seg[0]:k_seg[0] + min(128, k_seg[1])] = False  # and a first tile
+    mask = mask.cuda()
+    shut = (~mask).nonzero()[:, 0]
+    for i, bad in enumerate((math.nan, math.inf, -math.inf, torch.finfo(dtype).min, torch.finfo(dtype).max)):
+        k[shut[i::5]] = bad
+        v[shut[i::7]] = bad
+    clean_k, clean_v = k.clone(), v.clone()
+    clean_k[shut] = 0
+    clean_v[shut] = 0
+    want = check_cross(q, k, v, q_seg, k_seg, mask=mask)
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    pairs = ScenePairs(q_seg, k_seg)
+    one = cross_attention(q, k, v, pairs, mask=mask, return_lse=True)
+    two = cross_attention(q, clean_k, clean_v, pairs, mask=mask.to(torch.uint8), return_lse=True)
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+    d = normal(52, *q.shape, dtype=dtype)
+    dq, dk, dv = cross_attention_grad(d, q, k, v, *one, pairs, mask=mask)
+    assert not dk[shut].any() and not dv[shut].any()
+    empty = want.lse == -math.inf
+    assert empty.any() and not dq[empty.cuda()].any()
+
+
+@pytest.mark.parametrize("name", ["few rows on many", "many rows", "ragged"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_cross_growing_scores(name, dim):
+    # scores in the tens that grow along the keys: the running maximum moves
+    q, k, v, q_seg, k_seg = attention_inputs(60, lengths_case(name), 2, 1, dim, BF16, scale=3.0)
+    k *= torch.linspace(0.1, 2.0, len(k), device="cuda", dtype=torch.float32)[:, None, None].to(BF16)
+    check_cross(q, k, v, q_seg, k_seg)
+    check_cross(q, k, v, q_seg, k_seg, scale=0.001)
+
+
+def test_cross_infinities_and_nans_of_open_keys_and_queries():
+    from gsa_b200 import ScenePairs, cross_attention
+
+    for n_k in (60, 3000):  # one part, and split keys
+        q, k, v, q_seg, k_seg = attention_inputs(70, ([6], [n_k]), 1, 1, 32, BF16)
+        q[1] = math.nan
+        k[n_k // 2, 0, 3] = math.inf  # scores of +inf, or -inf, by the query's sign
+        v[n_k - 1, 0, 5] = math.inf
+        out, lse = cross_attention(q, k, v, ScenePairs(q_seg, k_seg), return_lse=True)
+        s = (q[:, 0].double() @ k[:, 0].double().T) * 32**-0.5
+        want = torch.softmax(s, 1) @ v[:, 0].double()
+        for r in range(6):
+            if s[r].isnan().any() or (s[r] == math.inf).any():
+                assert out[r].isnan().all() and lse[r].isnan().all()
+            else:
+                assert torch.equal(out[r, 0].isinf(), want[r].isinf())
+                rest = ~want[r].isinf()
+                assert torch.allclose(out[r, 0].double()[rest], want[r][rest], atol=0.05)
+        # nothing but -inf: no softmax
+        k[:, 0, :] = 0
+        k[:, 0, 0] = -math.inf
+        q[:] = 1
+        out, lse = cross_attention(q, k, v, ScenePairs(q_seg, k_seg), return_lse=True)
+        assert out.isnan().all()
+
+
+def test_cross_long_keys_of_many_scenes():
+    check_cross(*attention_inputs(80, ([1, 3, 1, 2], [9000, 1, 12000, 4097]), 4, 2, 64, FP16))
+
+
+def test_cross_writes_nothing_but_its_rows():
+    from gsa_b200 import ScenePairs, cross_attention
+
+    for lengths in (([130, 5], [300, 70]), ([1], [4000])):
+        q, k, v, q_seg, k_seg = attention_inputs(90, lengths, 2, 2, 40, BF16)
+        whole = torch.full((len(q) + 6, 4, 48), 7.0, dtype=BF16, device="cuda")
+        out = whole[3:-3, 1:3, :40]
+        cross_attention(q, k, v, ScenePairs(q_seg, k_seg), out=out)
+        assert torch.equal(out, cross_attention(q, k, v, ScenePairs(q_seg, k_seg)))
+        out.fill_(7.0)
+        assert (whole == 7.0).all()
+
+
+def test_cross_gradients_by_differences():
+    # the 64-bit output moved along a direction, against the kernel's gradient
+    q, k, v, q_seg, k_seg = attention_inputs(100, lengths_case("ragged"), 4, 2, 64, BF16)
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    pairs = ScenePairs(q_seg, k_seg)
+    d = normal(101, *q.shape, dtype=BF16)
+    out, lse = cross_attention(q, k, v, pairs, return_lse=True)
+    grads = cross_attention_grad(d, q, k, v, out, lse, pairs)
+    want = fo.Attention(q, k, v, q_seg, k_seg, dout=d)
+    for i, (name, t) in enumerate((("dq", q), ("dk", k), ("dv", v))):
+        step = torch.randn(t.shape, generator=torch.Generator().manual_seed(102 + i), dtype=torch.float64)
+        h = 1e-4
+        moved = []
+        for s in (1, -1):
+            xs = [x.double().cpu() + (s * h * step if x is t else 0) for x in (q, k, v)]
+            moved.append((fo.Attention(*xs, q_seg, k_seg).out * d.double().cpu()).sum())
+        slope = (moved[0] - moved[1]) / (2 * h)
+        bound = (getattr(want, name + "_off") * step.abs()).sum() + 1e-6 * slope.abs() + 1e-4
+        assert ((grads[i].double().cpu() * step).sum() - slope).abs() < bound, name
+
+
+def neighbor_ids(seed, lengths, width, kind):
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for n, m in zip(*lengths):
+        ids = torch.randint(0, max(m, 1), (n, width), generator=g)
+        if kind == "radius":  # ascending, then the first again
+            ids = ids.sort(1).values
+            found = torch.randint(0, width + 1, (n, 1), generator=g)
+            ids = torch.where(torch.arange(width) < found, ids, ids[:, :1])
+            ids = torch.where(found > 0, ids, 0)
+        else:  # absent entries of every sort, whole rows of them
+            bad = torch.rand(n, width, generator=g)
+            ids = torch.where(bad < 0.1, -1, ids)
+            ids = torch.where((bad > 0.1) & (bad < 0.2), m, ids)
+            ids = torch.where(bad > 0.95, 2**31 - 1, ids)
+            ids = torch.where((bad > 0.9) & (bad < 0.95), -(2**31), ids)
+            ids[::5] = -1
+        out.append(ids)
+    return torch.cat(out).int().cuda()
+
+
+def check_neighbors(q, k, v, ids, q_seg, k_seg, padded=True, scale=None, seed=78):
+    from gsa_b200 import ScenePairs, neighbor_attention, neighbor_attention_grad
+
+    pairs = ScenePairs(q_seg, k_seg)
+    out, lse = neighbor_attention(q, k, v, ids, pairs, padded=padded, scale=scale, return_lse=True)
+    dout = normal(seed, *q.shape, dtype=q.dtype)
+    want = fo.Attention(q, k, v, q_seg, k_seg, ids=ids, padded=padded, scale=scale, dout=dout)
+    want.close("out", out)
+    want.close("lse", lse)
+    got = neighbor_attention_grad(dout, q, k, v, ids, out, lse, pairs, padded=padded, scale=scale)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        want.close(name, t)
+    return want
+
+
+@pytest.mark.parametrize("kind,padded", [("radius", True), ("radius", False), ("absent", True), ("absent", False)])
+@pytest.mark.parametrize("dtype,dim,width", [(BF16, 32, 32), (FP16, 8, 3), (FP32, 24, 17), (BF16, 128, 8), (FP32, 128, 32),
+                                             (FP16, 72, 1), (FP32, 8, 5), (BF16, 16, 31)])
+def test_neighbors(dtype, dim, width, kind, padded):
+    lengths = lengths_case("ragged")
+    q, k, v, q_seg, k_seg = attention_inputs(110, lengths, 4, 2, dim, dtype)
+    check_neighbors(q, k, v, neighbor_ids(111, lengths, width, kind), q_seg, k_seg, padded)
+
+
+@pytest.mark.parametrize("heads,kv_heads,layout", [(1, 1, "packed"), (6, 1, "fused"), (5, 5, "heads first"), (12, 3, "packed")])
+@pytest.mark.parametrize("name", ["one", "few rows on many", "many rows", "no keys", "no queries"])
+def test_neighbors_heads_layouts_and_lengths(name, heads, kv_heads, layout):
+    lengths = lengths_case(name)
+    q, k, v, q_seg, k_seg = attention_inputs(120, lengths, heads, kv_heads, 40, FP32, layout)
+    check_neighbors(q, k, v, neighbor_ids(121, lengths, 9, "absent"), q_seg, k_seg)
+
+
+def test_neighbors_many_keys_and_one_key_for_all():
+    # keys of three digits of the sort, and a key that every entry names
+    lengths = ([3000], [300_000])
+    q, k, v, q_seg, k_seg = attention_inputs(130, lengths, 2, 1, 16, FP32)
+    ids = neighbor_ids(131, lengths, 7, "absent")
+    from gsa_b200 import ScenePairs, neighbor_attention, neighbor_attention_grad
+
+    pairs = ScenePairs(q_seg, k_seg)
+    out, lse = neighbor_attention(q, k, v, ids, pairs, return_lse=True)
+    d = normal(132, *q.shape)
+    _, dk, dv = neighbor_attention_grad(d, q, k, v, ids, out, lse, pairs)
+    # the same on the keys that are named, packed
+    named, at = ids[(ids >= 0) & (ids < 300_000)].long().unique(return_inverse=True)
+    packed = torch.full_like(ids, -1)
+    packed[(ids >= 0) & (ids < 300_000)] = at.int()
+    want = fo.Attention(q, k[named], v[named], q_seg, [0, len(named)], ids=packed, dout=d)
+    want.close("out", out)
+    want.close("dk", dk[named])
+    want.close("dv", dv[named])
+    rest = torch.ones(300_000, dtype=torch.bool, device="cuda")
+    rest[named] = False
+    assert not dk[rest].any() and not dv[rest].any()
+    q, k, v, q_seg, k_seg = attention_inputs(133, ([900], [5]), 2, 1, 16, FP32)
+    check_neighbors(q, k, v, torch.full((900, 4), 3, dtype=torch.int32, device="cuda"), q_seg, k_seg, padded=False)
+
+
+def test_neighbor_gradients_by_differences():
+    from gsa_b200 import ScenePairs, neighbor_attention, neighbor_attention_grad
+
+    lengths = lengths_case("ragged")
+    q, k, v, q_seg, k_seg = attention_inputs(140, lengths, 2, 2, 16, FP32)
+    ids = neighbor_ids(141, lengths, 6, "radius")
+    pairs = ScenePairs(q_seg, k_seg)
+    d = normal(142, *q.shape)
+    out, lse = neighbor_attention(q, k, v, ids, pairs, return_lse=True)
+    grads = neighbor_attention_grad(d, q, k, v, ids, out, lse, pairs)
+    h = 2.0**-8
+    for i, t in enumerate((q, k, v)):
+        step = normal(143 + i, *t.shape)
+        moved = [(neighbor_attention(*(x + s * h * step if x is t else x for x in (q, k, v)), ids, pairs).double()
+                  * d.double()).sum() for s in (1, -1)]
+        slope = ((moved[0] - moved[1]) / (2 * h)).item()
+        got = (grads[i].double() * step.double()).sum().item()
+        # 32-bit outputs over 2 h: 2^-18 of sum |d| / h; third derivatives: h^2 of sum |d|
+        assert abs(got - slope) < d.abs().double().sum().item() * (2.0**-18 / h + h * h)
+
+
+# ---------------------------------------------------------------------------
+# how programs call them
+
+
+def both(kind, lengths=([130, 64, 1], [70, 129, 900]), dim=32, dtype=BF16, seed=150):
+    """A forward and a gradient call of either attention on the same rows."""
+    from gsa_b200 import ScenePairs, attention as at
+
+    q, k, v, q_seg, k_seg = attention_inputs(seed, lengths, 4, 2, dim, dtype)
+    pairs = ScenePairs(q_seg, k_seg)
+    ids = neighbor_ids(seed + 5, lengths, 8, "radius")
+    d = normal(seed + 6, *q.shape, dtype=dtype)
+    if kind == "cross":
+        def forward(**kw):
+            return at.cross_attention(q, k, v, pairs, **kw)
+
+        def backward(out, lse):
+            return at.cross_attention_grad(d, q, k, v, out, lse, pairs)
+    else:
+        def forward(**kw):
+            return at.neighbor_attention(q, k, v, ids, pairs, **kw)
+
+        def backward(out, lse):
+            return at.neighbor_attention_grad(d, q, k, v, ids, out, lse, pairs)
+    return (q, k, v), d, forward, backward
+
+
+@pytest.mark.parametrize("kind", ["cross", "neighbor"])
+def test_the_same_bits_again(kind):
+    _, _, forward, backward = both(kind, ([400, 9], [1900, 300]))
+    out, lse = forward(return_lse=True)
+    first = backward(out, lse)
+    for _ in range(5):
+        o, m = forward(return_lse=True)
+        assert torch.equal(o, out) and torch.equal(m, lse)
+        assert all(torch.equal(a, b) for a, b in zip(first, backward(o, m)))
+
+
+@pytest.mark.parametrize("kind", ["cross", "neighbor"])
+def test_autograd_is_the_gradient_call(kind):
+    leaves, d, forward, backward = both(kind)
+    out, lse = forward(return_lse=True)
+    want = backward(out, lse)
+    for t in leaves:
+        t.requires_grad_()
+    got = forward()
+    assert torch.equal(got, out)
+    got.backward(d)
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    for t in leaves:
+        t.grad = None
+    forward().float().sum().backward()  # an expanded gradient
+    assert all(t.grad is not None and t.grad.isfinite().all() for t in leaves)
+    with torch.no_grad():
+        assert not forward().requires_grad
+
+
+@pytest.mark.parametrize("kind", ["cross", "neighbor"])
+def test_streams_and_captured_graphs(kind):
+    leaves, d, forward, backward = both(kind, ([5, 300], [3000, 70]))
+    out, lse = forward(return_lse=True)
+    want = backward(out, lse)
+    torch.cuda.synchronize()
+    # two streams at once
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                o, m = forward(return_lse=True)
+                results.append((o, m, *backward(o, m)))
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(a, b) for a, b in zip(got, (out, lse, *want)))
+    # two captured graphs, replayed at once on new inputs
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o, m = forward(return_lse=True)
+            got = (o, m, *backward(o, m))
+        graphs.append((g, got))
+    for t in leaves:
+        t.copy_(t.flip(-1) * 0.5)
+    out, lse = forward(return_lse=True)
+    want = backward(out, lse)
+    torch.cuda.synchronize()
+    for s, (g, _) in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    for _, got in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(got, (out, lse, *want)))
+
+
+def test_attention_refuses():
+    from gsa_b200 import ScenePairs, attention as at
+
+    q, k, v, q_seg, k_seg = attention_inputs(160, ([5, 4], [6, 3]), 4, 2, 16, BF16)
+    pairs = ScenePairs(q_seg, k_seg)
+    ids = torch.zeros(9, 3, dtype=torch.int32, device="cuda")
+    out, lse = at.cross_attention(q, k, v, pairs, return_lse=True)
+    odd = normal(1, 9 * 64 + 1, dtype=BF16)[1:].view(9, 4, 16)
+    bad = [dict(q=q.float()), dict(q=q.double()), dict(q=q.half()), dict(k=k.half()), dict(v=v[:8]), dict(q=q[:8]),
+           dict(q=q[:, :3]), dict(q=q[..., :12], k=k[..., :12], v=v[..., :12]), dict(q=odd), dict(q=q.cpu()),
+           dict(v=v[:, :1]), dict(k=k[..., :8]), dict(q=q[0]), dict(pairs=None), dict(scale=0.0), dict(scale=-1.0),
+           dict(scale=math.nan), dict(pairs=ScenePairs([0, 9], [0, 8])), dict(out=out[:8]), dict(out=out.float()),
+           dict(out=q), dict(out=out[:, :1].expand(9, 4, 16)), dict(out=odd)]
+    for change in bad + [dict(mask=torch.ones(8, dtype=torch.bool, device="cuda")), dict(mask=torch.ones(9)),
+                         dict(mask=torch.ones(9, device="cuda"))]:
+        args = dict(q=q, k=k, v=v, pairs=pairs)
+        args.update(change)
+        with pytest.raises(ValueError):
+            at.cross_attention(**args)
+    for change in bad[1:] + [dict(rows=ids[:8]), dict(rows=ids.long()), dict(rows=ids[:, :0]), dict(rows=ids.cpu()),
+                             dict(rows=torch.zeros(9, 33, dtype=torch.int32, device="cuda")), dict(rows=ids.T)]:
+        if "q" in change and change["q"].dtype == FP16:
+            continue  # q alone differs from k: covered by k
+        args = dict(q=q, k=k, v=v, rows=ids, pairs=pairs)
+        args.update(change)
+        with pytest.raises(ValueError):
+            at.neighbor_attention(**args)
+    for change in [dict(dout=q[:8]), dict(dout=q.float()), dict(out=out[:8]), dict(lse=lse.double()), dict(lse=lse[:8]),
+                   dict(lse=lse.T), dict(dout=odd)]:
+        args = dict(dout=q, q=q, k=k, v=v, out=out, lse=lse, pairs=pairs)
+        args.update(change)
+        with pytest.raises(ValueError):
+            at.cross_attention_grad(**args)
+        with pytest.raises(ValueError):
+            at.neighbor_attention_grad(rows=ids, **args)
