@@ -26,6 +26,31 @@
 namespace gsa {
 namespace {
 
+constexpr int kBlock = 128;
+template <typename T, int kN>
+__device__ __forceinline__ void load_keys(const Chunks& c, uint32_t tile,
+                                          const T* base, long long row,
+                                          const unsigned char* mask, int k0,
+                                          int n) {
+  if (!c.live) return;
+  for (int i = c.row; i < kN; i += c.step) {
+    const int r = k0 + i;
+    const bool there = c.data && r < n && (!mask || __ldg(mask + r));
+    const T* from = there ? base + r * row + c.chunk * 8 : base;
+    tc::copy16(tile + tc::tile_offset(kN, i, c.chunk), from, there);
+  }
+}
+template <int kN>
+__device__ __forceinline__ void block_words(uint32_t* words,
+                                          const unsigned char* mask, int k0,
+                                          int n) {
+  if (threadIdx.x < kN) {
+    const int r = k0 + (int)threadIdx.x;
+    const bool open = r < n && (!mask || __ldg(mask + r));
+    const uint32_t w = __ballot_sync(kFull, open);
+    if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = w;
+  }
+}
 constexpr int kWalk = 64;    // rows of a walked tile
 constexpr int kStages = 3;
 
@@ -62,7 +87,7 @@ __device__ __forceinline__ float ds_bits(int keys) {
 }
 
 template <typename T, int kDim, bool kKeysPass>
-__global__ void __launch_bounds__(kThreads, Shape<kDim, kKeysPass>::kBlocks)
+__global__ void __launch_bounds__(kBlock, Shape<kDim, kKeysPass>::kBlocks)
     cross_backward_kernel(const __grid_constant__ CrossArgs a) {
   using S = Shape<kDim, kKeysPass>;
   extern __shared__ uint8_t smem_raw[];
@@ -113,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kKeysPass>::kBlocks)
       tc::barrier_init(bar_a, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Chunks c = chunks_of(a.dim);
+    const Chunks c = chunks_of(a.dim, tid, kBlock);
     const T* q = static_cast<const T*>(a.q) + q0 * a.q_row +
                  (long long)hk * a.group * a.q_head;
     const T* d = static_cast<const T*>(a.dout) + q0 * a.d_row +
@@ -150,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kKeysPass>::kBlocks)
         } else {
           load_keys<T, kWalk>(c, t1, k, a.k_row, mask, at, nk);
           load_keys<T, kWalk>(c, t2, v, a.v_row, mask, at, nk);
-          key_words<kWalk>(words[t & 3], mask, at, nk);
+          block_words<kWalk>(words[t & 3], mask, at, nk);
         }
       }
       tc::copy_commit();
@@ -179,12 +204,10 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kKeysPass>::kBlocks)
     tc::fence_after();
     tmem = tmem_at;
     auto scores = [&](int t) {
-      tc::product_by_columns<T>(tmem + S::kS, x1, kRows,
-                                y1 + (t % kStages) * S::kTile, kWalk, kWalk,
-                                steps);
-      tc::product_by_columns<T>(tmem + S::kDp, x2, kRows,
-                                y2 + (t % kStages) * S::kTile, kWalk, kWalk,
-                                steps);
+      tc::product_by_columns<T, kRows, kWalk, kDim / 16>(
+          tmem + S::kS, x1, y1 + (t % kStages) * S::kTile, steps);
+      tc::product_by_columns<T, kRows, kWalk, kDim / 16>(
+          tmem + S::kDp, x2, y2 + (t % kStages) * S::kTile, steps);
       tc::commit(bar_s);
     };
     if (tid == 0) scores(0);
@@ -249,11 +272,11 @@ __global__ void __launch_bounds__(kThreads, Shape<kDim, kKeysPass>::kBlocks)
         if (!S::kOverwrite && t + 1 < nt) scores(t + 1);
         const uint32_t t1 = y1 + (t % kStages) * S::kTile,
                        t2 = y2 + (t % kStages) * S::kTile;
-        tc::product_by_rows<T>(tmem + S::kOut1, tmem + S::kDs, t1, kWalk,
-                               steps * 16, kWalk / 16, t > 0);
+        tc::product_by_rows<T, kWalk>(tmem + S::kOut1, tmem + S::kDs, t1,
+                                      steps * 16, t > 0);
         if constexpr (kKeysPass)
-          tc::product_by_rows<T>(tmem + S::kOut2, tmem + S::kP, t2, kWalk,
-                                 steps * 16, kWalk / 16, t > 0);
+          tc::product_by_rows<T, kWalk>(tmem + S::kOut2, tmem + S::kP, t2,
+                                        steps * 16, t > 0);
         tc::commit(bar_a);
         if (S::kOverwrite && t + 1 < nt) {
           ok = ok && tc::barrier_wait(bar_a, t & 1);
@@ -414,7 +437,7 @@ cudaError_t launch_pass(CrossArgs a, const Plan& p, cudaStream_t s) {
   if (e) return e;
   count_launches(1);
   cross_backward_kernel<T, kDim, kKeysPass>
-      <<<(unsigned)grid, kThreads, S::kSmem, s>>>(a);
+      <<<(unsigned)grid, kBlock, S::kSmem, s>>>(a);
   if (a.splits > 1) {
     const long long n =
         kKeysPass ? a.n_k * a.kv_heads * a.dim : a.n_q * a.heads * a.dim;

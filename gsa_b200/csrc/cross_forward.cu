@@ -6,286 +6,393 @@
 //
 // over the scene's open keys; a row without any gives 0 and lse = -inf.
 //
-// A block owns 128 packed query rows and walks the keys in tiles.  Products
-// run on tcgen05: S = Q K^T into tensor memory; every thread takes one row of
-// it into registers, keeps the running maximum and sum in 32 bits, and writes
-// P = exp(S - max), rounded to the inputs' type for the second product (half
-// a step, 2^-8 for bf16, on weights that are summed in 32 bits), back to
-// tensor memory, from where O += P V takes it.  The maximum that P is taken
-// against may lag the true one by a factor of 2^8, so that O is rescaled only
-// when it grew by more.
+// A block owns 128 packed query rows, a row per thread, and walks the keys in
+// tiles of 128.  A fifth warp issues the products (tcgen05), a sixth loads the
+// tiles (TMA): one warp for both took longer over a tile than its rows did.
+// S = Q K^T comes from tensor memory into registers, the running maximum and
+// sum are kept in 32 bits, and P = exp(S - max), rounded to the inputs' type
+// for the second product (half a step, 2^-8 for bf16, on weights that are
+// summed in 32 bits), goes back to tensor memory, from where O += P V takes
+// it.  The maximum that P is taken against may lag the true one by a factor of
+// 2^8, so that O is rescaled only when it grew by more.  Value rows of shut or
+// absent keys are cleared in shared memory before their product, so that
+// whatever lies there takes no part.
 //
-// What bounds it: the exponentials (16 a clock on an SM) up to a head of 128
-// elements, where the two products take as long.  Tensor memory (256 columns)
-// and shared memory (at most 96 KB) leave room for two blocks on an SM, so one
-// block's exponentials run beside the other's products.  Where there are too
-// few row tiles to fill the GPU, the keys are split among blocks and the
-// parts joined by their lse.
+// What bounds it: a row's chain of waits, softmax and waits again, which only
+// another block's work can fill; two blocks share an SM (256 columns of
+// tensor memory, at most 97 KB of shared memory each).  Below that lie the
+// exponentials (16 a clock on an SM; a quarter are polynomials in the
+// multiply-add units) up to a head of 128, where the products take as long.
+// 8 x 24,000 queries on 6,000 keys, 4 heads of 128: 2.46 ms, 960 TFLOP/s;
+// 8 x 6,000 on 1,500, 8 heads of 64: 250 us, 590 TFLOP/s.  Tiles of 64 keys
+// with four blocks on an SM took 253 to 274 us and 2.7 to 2.8 ms, two threads
+// per row 268 us and 2.68 ms.
+//
+// Where there are too few row tiles to fill the GPU, the keys are split among
+// blocks and the parts joined by their lse.
 #include "cross.cuh"
 
 namespace gsa {
 namespace {
 
-// Head size up to kDim (64 or 128); keys per tile.
+constexpr int kKeys = 128;  // keys of a tile
+
+// Head size up to kDim (64 or 128).  The larger one has room for one tile of
+// keys and values in shared memory, and for P in tensor memory only where S
+// was: its next scores wait for the product that reads P.
 template <int kDim>
 struct Shape {
-  static constexpr int kKeys = kDim == 64 ? 128 : 64;
-  static constexpr int kQ = kRows * kDim * 2;      // bytes
-  static constexpr int kTileBytes = kKeys * kDim * 2;
-  static constexpr int kSmem = 1024 + kQ + 4 * kTileBytes;
+  static constexpr int kStages = kDim == 64 ? 2 : 1;
+  static constexpr bool kOverwrite = kDim == 128;
+  static constexpr int kQ = kRows * kDim * 2;  // bytes
+  static constexpr int kTile = kKeys * kDim * 2;
+  static constexpr int kSmem = 1024 + kQ + 2 * kStages * kTile;
   static constexpr uint32_t kColumns = 256;
-  static constexpr uint32_t kS = 0, kP = kKeys, kO = kKeys + kKeys / 2;
-  static_assert(kO + kDim <= 256, "tensor memory");
+  static constexpr uint32_t kS = 0, kP = kOverwrite ? 0 : 128,
+                            kO = kOverwrite ? 128 : 192;
+  static_assert(kO + kDim == kColumns, "tensor memory");
 };
+
+struct Maps {
+  CUtensorMap k, v;
+};
+
+enum Bar {
+  kKeysFull = 0,    // [stage] the keys are there
+  kKeysFree = 2,    // [stage] the scores that read them are complete
+  kValuesFull = 4,  // [stage]
+  kValuesFree = 6,  // [stage]
+  kValuesRaw = 8,   // values loaded, rows to be cleared
+  kScores = 9,      // S is complete
+  kScoresRead = 10,  // S is in registers (a count per warp of rows)
+  kWeights = 11,    // P is there (a count per warp of rows)
+  kOutput = 12,     // O += P V is complete
+  kBars = 13
+};
+
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 template <typename T, int kDim>
 __global__ void __launch_bounds__(kThreads, 2)
-    cross_forward_kernel(const __grid_constant__ CrossArgs a) {
+    cross_forward_kernel(const __grid_constant__ CrossArgs a,
+                         const __grid_constant__ Maps maps) {
   using S = Shape<kDim>;
-  constexpr int kKeys = S::kKeys;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[2];
+  __shared__ uint64_t bars[kBars];
   __shared__ uint32_t tmem_at;
-  __shared__ uint32_t words[4][kKeys / 32];
 
   unsigned unit = blockIdx.x;
-  const int tile = unit % a.tiles;
+  const int r0 = unit % a.tiles * kRows;
   unit /= a.tiles;
   const int split = unit % a.splits;
   unit /= a.splits;
   const int hk = unit % a.kv_heads;
   const int scene = unit / a.kv_heads;
-  const int q0 = a.q_seg[scene], k0 = a.k_seg[scene];
-  const int n = (a.q_seg[scene + 1] - q0) * a.group;  // packed rows
-  const int nk = a.k_seg[scene + 1] - k0;
-  const int r0 = tile * kRows;
+  const int q0 = __ldg(a.q_seg + scene), k0 = __ldg(a.k_seg + scene);
+  const int n = (__ldg(a.q_seg + scene + 1) - q0) * a.group;  // packed rows
+  const int nk = __ldg(a.k_seg + scene + 1) - k0;
   if (r0 >= n) return;
   int begin, end;
   share((nk + kKeys - 1) / kKeys, a.splits, split, &begin, &end);
   const int nt = end - begin;
 
-  const int tid = threadIdx.x, warp = tid >> 5;
-  const uint32_t smem =
-      (tc::smem_address(smem_raw) + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_tile = smem, k_tile = smem + S::kQ,
-                 v_tile = k_tile + 2 * S::kTileBytes;
-  const uint32_t bar_s = tc::smem_address(&bars[0]),
-                 bar_o = tc::smem_address(&bars[1]);
-  const int steps = (a.dim + 15) / 16;
-
-  const int r = r0 + tid;
-  const bool live = r < n;
-  const bool busy = r0 + warp * 32 < n;  // the warp holds rows
-  bool ok = true;
-  float m = -kInf, l = 0.f;
-  uint32_t seen = 0;
+                 v_tile = k_tile + S::kStages * S::kTile;
+  const uint32_t bar0 = tc::smem_address(bars);
+  const unsigned char* mask = a.mask ? a.mask + k0 : nullptr;
   uint32_t tmem = 0;
-
+  bool ok = true;
+  auto bar = [&](int which) { return bar0 + which * 8; };
+  auto wait = [&](int which, int phase) {
+    if (ok) ok = tc::barrier_wait(bar0 + which * 8, phase & 1);
+  };
   if (nt > 0) {
-    if (warp == 0) tc::tmem_alloc(tc::smem_address(&tmem_at), S::kColumns);
-    if (tid == 0) {
-      tc::barrier_init(bar_s, 1);
-      tc::barrier_init(bar_o, 1);
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    const Chunks c = chunks_of(a.dim);
-    const T* q = static_cast<const T*>(a.q) + q0 * a.q_row +
-                 (long long)hk * a.group * a.q_head;
-    const T* k = static_cast<const T*>(a.k) + k0 * a.k_row + hk * a.k_head;
-    const T* v = static_cast<const T*>(a.v) + k0 * a.v_row + hk * a.v_head;
-    const unsigned char* mask = a.mask ? a.mask + k0 : nullptr;
-    auto load_k = [&](int t) {
-      if (t < nt) {
-        load_keys<T, kKeys>(c, k_tile + (t & 1) * S::kTileBytes, k, a.k_row,
-                            mask, (begin + t) * kKeys, nk);
-        key_words<kKeys>(words[t & 3], mask, (begin + t) * kKeys, nk);
+    if (warp == 4) {
+      tc::tmem_alloc(tc::smem_address(&tmem_at), S::kColumns);
+      if (lane == 0) {
+        for (int i = 0; i < kBars; ++i)
+          tc::barrier_init(bar(i), i == kScoresRead || i == kWeights ? 4 : 1);
+        tc::barriers_ready();
       }
+    } else if (warp < 4) {
+      load_packed<T, kRows>(
+          chunks_of(a.dim, tid, kRows), q_tile,
+          static_cast<const T*>(a.q) + q0 * a.q_row +
+              (long long)hk * a.group * a.q_head,
+          a.q_row, a.q_head, a.group, r0, n);
       tc::copy_commit();
-    };
-    auto load_v = [&](int t) {
-      if (t < nt)
-        load_keys<T, kKeys>(c, v_tile + (t & 1) * S::kTileBytes, v, a.v_row,
-                            mask, (begin + t) * kKeys, nk);
-      tc::copy_commit();
-    };
-    load_packed<T, kRows>(c, q_tile, q, a.q_row, a.q_head, a.group, r0, n);
-    load_k(0);
-    load_k(1);
-    load_v(0);
-    tc::copy_wait<2>();
-    tc::fence_shared();
+      tc::copy_wait<0>();
+      tc::fence_shared();
+    }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     tmem = tmem_at;
-    auto scores = [&](int t) {
-      tc::product_by_columns<T>(tmem + S::kS, q_tile, kRows,
-                                k_tile + (t & 1) * S::kTileBytes, kKeys, kKeys,
-                                steps);
-      tc::commit(bar_s);
-    };
-    if (tid == 0) scores(0);
-    const uint32_t mine = tmem + ((uint32_t)warp << 21);  // the warp's rows
+  }
 
+  if (warp == 5) {
+    const int panels = a.dim > 64 ? 2 : 1;
+    int cleared = 0;
     for (int t = 0; t < nt; ++t) {
-      uint32_t s[kKeys];
-      ok = ok && tc::barrier_wait(bar_s, t & 1);
+      const int stage = t % S::kStages, round = t / S::kStages;
+      const int at = (begin + t) * kKeys;
+      const uint32_t kt = k_tile + stage * S::kTile,
+                     vt = v_tile + stage * S::kTile;
+      uint32_t open[kKeys / 32];
+      key_words<kKeys>(open, mask, at, nk);
+      const bool whole =
+          (open[0] & open[1] & open[2] & open[3]) == 0xffffffffu;
+      const int full = whole ? kValuesFull + stage : kValuesRaw;
+      if (round > 0) wait(kKeysFree + stage, round - 1);
       __syncwarp();
+      if (tc::elect()) {
+        tc::barrier_expect(bar(kKeysFull + stage), panels * kKeys * 128);
+        for (int p = 0; p < panels; ++p)
+          tc::copy_box(kt + p * kKeys * 128, &maps.k, bar(kKeysFull + stage),
+                       p * 64, hk, k0 + at);
+      }
+      if (round > 0) wait(kValuesFree + stage, round - 1);
+      __syncwarp();
+      if (tc::elect()) {
+        tc::barrier_expect(bar(full), panels * kKeys * 128);
+        for (int p = 0; p < panels; ++p)
+          tc::copy_box(vt + p * kKeys * 128, &maps.v, bar(full), p * 64, hk,
+                       k0 + at);
+      }
+      if (!whole) {
+        wait(kValuesRaw, cleared++);
+        __syncwarp();
+        clear_rows<kKeys>(vt, panels, open);
+        tc::fence_shared();
+        __syncwarp();
+        if (lane == 0) tc::barrier_arrive(bar(kValuesFull + stage));
+      }
+    }
+  } else if (warp == 4) {
+    const int steps = (a.dim + 15) / 16;
+    auto scores = [&](int t) {  // its keys are there
       tc::fence_after();
-      if (busy) {
+      __syncwarp();
+      if (tc::elect()) {
+        tc::product_by_columns<T, kRows, kKeys, kDim / 16>(
+            tmem + S::kS, q_tile, k_tile + t % S::kStages * S::kTile, steps);
+        tc::commit(bar(kScores));
+        tc::commit(bar(kKeysFree + t % S::kStages));
+      }
+      __syncwarp();
+    };
+    if (nt > 0) {
+      wait(kKeysFull, 0);
+      scores(0);
+    }
+    for (int t = 0; t < nt; ++t) {
+      const int stage = t % S::kStages;
+      const bool more = t + 1 < nt;
+      if (more)
+        wait(kKeysFull + (t + 1) % S::kStages, (t + 1) / S::kStages);
+      if (!S::kOverwrite && more) {
+        wait(kScoresRead, t);
+        scores(t + 1);
+      }
+      wait(kValuesFull + stage, t / S::kStages);
+      wait(kWeights, t);
+      tc::fence_after();
+      __syncwarp();
+      if (tc::elect()) {
+        tc::product_by_rows<T, kKeys>(tmem + S::kO, tmem + S::kP,
+                                      v_tile + stage * S::kTile, steps * 16,
+                                      t > 0);
+        tc::commit(bar(kOutput));
+        tc::commit(bar(kValuesFree + stage));
+      }
+      __syncwarp();
+      if (S::kOverwrite && more) {
+        wait(kOutput, t);
+        scores(t + 1);
+      }
+    }
+  } else {
+    const int r = r0 + tid;
+    const bool live = r < n;
+    const bool busy = r0 + warp * 32 < n;  // the warp holds rows
+    const uint32_t mine = tmem + ((uint32_t)warp << 21);  // the warp's rows
+    float m = -kInf, l = 0.f;
+    bool seen = false;  // an open key
+    if (!busy) {
+      for (int t = 0; t < nt; ++t) {
+        wait(kScores, t);
+        if (lane == 0 && !S::kOverwrite) tc::barrier_arrive(bar(kScoresRead));
+        // no arrival for the next tile before this one's phase is complete
+        if (t > 0) wait(kOutput, t - 1);
+        if (lane == 0) tc::barrier_arrive(bar(kWeights));
+        __syncwarp();
+      }
+    } else {
+      const uint64_t scale2 = tc::pair(a.scale_log2e, a.scale_log2e);
+      for (int t = 0; t < nt; ++t) {
+        uint32_t s[kKeys];
+        wait(kScores, t);
+        __syncwarp();
+        tc::fence_after();
 #pragma unroll
         for (int i = 0; i < kKeys; i += 32) tc::load32(mine + S::kS + i, s + i);
         tc::wait_load();
-      }
-      load_k(t + 2);
-      tc::copy_wait<2>();  // the next keys are there
-      tc::fence_shared();
-      tc::fence_before();
-      __syncthreads();
-      if (tid == 0 && t + 1 < nt) {
-        tc::fence_after();
-        scores(t + 1);
-      }
-      uint32_t p[kKeys / 2];
-      float rescale = 1.f;
-      if (busy) {
-        float top = -kInf;
-#pragma unroll
-        for (int w = 0; w < kKeys / 32; ++w) {
-          const uint32_t open = words[t & 3][w];
-          seen |= open;
-          if (open != 0xffffffffu) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((open >> i) & 1)) s[w * 32 + i] = 0xff800000u;
-          }
+        if (!S::kOverwrite) {
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::barrier_arrive(bar(kScoresRead));
         }
+        const int at = (begin + t) * kKeys;
+        if (mask || at + kKeys > nk) {
+          uint32_t open[kKeys / 32];
+          key_words<kKeys>(open, mask, at, nk);
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) top = fmaxf(top, __uint_as_float(s[i]));
-        top *= a.scale_log2e;
-        if (top > m + 8.f || m == -kInf) {
+          for (int w = 0; w < kKeys / 32; ++w) {
+            seen |= open[w] != 0;
+            if (open[w] != 0xffffffffu) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((open[w] >> i) & 1)) s[w * 32 + i] = 0xff800000u;
+            }
+          }
+        } else {
+          seen = true;
+        }
+        // The maximum, NaN if any score is; an infinite one has no softmax.
+        float tops[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          tops[i] = max3(__uint_as_float(s[3 * i]),
+                         __uint_as_float(s[3 * i + 1]),
+                         __uint_as_float(s[3 * i + 2]));
+#pragma unroll
+        for (int i = 12; i < kKeys; i += 2)
+          tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], __uint_as_float(s[i]),
+                                    __uint_as_float(s[i + 1]));
+        float top = max3(tops[0], tops[1], max3(tops[2], tops[3], tops[3])) *
+                    a.scale_log2e;
+        if (top == kInf) top = __int_as_float(0x7fffffff);
+        float rescale = 1.f;
+        if (!(top <= m + 8.f) || m == -kInf) {
           rescale = m == -kInf ? 0.f : exp2_fast(m - top);
           m = top;
           l *= rescale;
         }
         const float shift = m == -kInf ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t shift2 = tc::pair(-shift, -shift);
+        uint64_t sum[2] = {0, 0};
+        // P and its sum, a half at a time; P's place and O are free once the
+        // last tile's product is complete, which the first half hides
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 2) {
-          const float x = exp2_fast(
-              fmaf(__uint_as_float(s[i]), a.scale_log2e, -shift));
-          const float y = exp2_fast(
-              fmaf(__uint_as_float(s[i + 1]), a.scale_log2e, -shift));
-          sum[i & 2] += x;
-          sum[(i & 2) + 1] += y;
-          p[i / 2] = pack2<T>(x, y);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      }
-      if (t > 0) {
-        ok = ok && tc::barrier_wait(bar_o, (t - 1) & 1);
-        __syncwarp();
-        tc::fence_after();
-      }
-      load_v(t + 1);
-      if (busy) {
-        if (t > 0 && __any_sync(kFull, rescale != 1.f)) {
-          for (int i = 0; i < steps * 16; i += 16) {
-            uint32_t o[16];
-            tc::load16(mine + S::kO + i, o);
-            tc::wait_load();
+        for (int c = 0; c < kKeys; c += kKeys / 2) {
+          uint32_t p[kKeys / 4];
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              o[e] = __float_as_uint(__uint_as_float(o[e]) * rescale);
-            tc::store16(mine + S::kO + i, o);
+          for (int i = 0; i < kKeys / 2; i += 2) {
+            const uint64_t x =
+                tc::fma2(tc::pair(__uint_as_float(s[c + i]),
+                                  __uint_as_float(s[c + i + 1])),
+                         scale2, shift2);
+            float u0, u1;
+            if ((i >> 1) % 4 == 3) {
+              exp2_polynomial(x, &u0, &u1);
+            } else {
+              tc::unpair(x, &u0, &u1);
+              u0 = exp2_fast(u0);
+              u1 = exp2_fast(u1);
+            }
+            sum[(i >> 1) & 1] = tc::add2(sum[(i >> 1) & 1], tc::pair(u0, u1));
+            p[i / 2] = pack2<T>(u0, u1);
           }
-        }
+          if (c == 0 && t > 0) {
+            wait(kOutput, t - 1);
+            __syncwarp();
+            tc::fence_after();
+            if (__any_sync(kFull, rescale != 1.f)) {
+              for (int i = 0; i < a.dim; i += 8) {
+                uint32_t o[8];
+                tc::load8(mine + S::kO + i, o);
+                tc::wait_load();
 #pragma unroll
-        for (int i = 0; i < kKeys / 2; i += 16)
-          tc::store16(mine + S::kP + i, p + i);
+                for (int e = 0; e < 8; ++e)
+                  o[e] = __float_as_uint(__uint_as_float(o[e]) * rescale);
+                tc::store8(mine + S::kO + i, o);
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kKeys / 4; i += 16)
+            tc::store16(mine + S::kP + c / 2 + i, p + i);
+        }
+        float u0, u1;
+        tc::unpair(tc::add2(sum[0], sum[1]), &u0, &u1);
+        l += u0 + u1;
         tc::wait_store();
-      }
-      tc::copy_wait<2>();  // this tile's values are there
-      tc::fence_shared();
-      tc::fence_before();
-      __syncthreads();
-      if (tid == 0) {
-        tc::fence_after();
-        tc::product_by_rows<T>(tmem + S::kO, tmem + S::kP,
-                               v_tile + (t & 1) * S::kTileBytes, kKeys,
-                               steps * 16, kKeys / 16, t > 0);
-        tc::commit(bar_o);
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::barrier_arrive(bar(kWeights));
       }
     }
-    ok = ok && tc::barrier_wait(bar_o, (nt - 1) & 1);
-    __syncwarp();
-    tc::fence_after();
-    tc::copy_wait<0>();
-  }
+    if (nt > 0) {
+      wait(kOutput, nt - 1);
+      __syncwarp();
+      tc::fence_after();
+    }
 
-  const int qr = live ? r / a.group : 0;
-  const int h = hk * a.group + (live ? r - qr * a.group : 0);
-  const long long row = q0 + qr;
-  const float inv = seen ? 1.f / l : 0.f;
-  if (a.splits == 1) {
-    T* o = static_cast<T*>(a.o) + row * a.o_row + h * a.o_head;
-    if (live && a.lse)
-      a.lse[row * a.heads + h] = seen ? (m + log2f(l)) * kLn2 : -kInf;
     if (busy) {
-      for (int i = 0; i < a.dim; i += 16) {
-        uint32_t x[16];
-        if (seen) {
-          __syncwarp();
-          tc::load16(tmem + ((uint32_t)warp << 21) + S::kO + i, x);
-          tc::wait_load();
-        }
-        float f[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          f[e] = seen ? __uint_as_float(x[e]) * inv : 0.f;
-        if (live) {
-          *reinterpret_cast<uint4*>(o + i) = Vec<T>::pack(f);
-          if (i + 8 < a.dim)
-            *reinterpret_cast<uint4*>(o + i + 8) = Vec<T>::pack(f + 8);
-        }
+      const int qr = live ? r / a.group : 0;
+      const int h = hk * a.group + (live ? r - qr * a.group : 0);
+      const long long row = q0 + qr;
+      const long long at =
+          a.splits == 1 ? row * a.heads + h
+                        : ((long long)split * a.n_q + row) * a.heads + h;
+      // A part whose scores are all -inf counts for nothing beside others,
+      // but a row of nothing else has no softmax (NaN): such a part is told
+      // by a finite lse below all others.
+      const bool none = !seen || (a.splits > 1 && l == 0.f);
+      const float inv = none ? 0.f : 1.f / l;
+      if (live) {
+        const float lse2 = seen ? m + log2f(l) : -kInf;
+        if (a.splits > 1)
+          a.part_lse[at] = seen && none ? -3.0e38f : lse2;
+        else if (a.lse)
+          a.lse[at] = lse2 * kLn2;
       }
-    }
-  } else {
-    // A part whose scores are all -inf counts for nothing beside others, but
-    // a row of nothing else has no softmax (NaN): it is told apart by a
-    // finite lse below all others.
-    const long long at = ((long long)split * a.n_q + row) * a.heads + h;
-    const bool none = !seen || l == 0.f;
-    if (live)
-      a.part_lse[at] = !seen ? -kInf : l == 0.f ? -3.0e38f : m + log2f(l);
-    if (busy) {
-      for (int i = 0; i < a.dim; i += 16) {
-        uint32_t x[16];
+      for (int i = 0; i < a.dim; i += 8) {
+        uint32_t x[8];
+        float f[8];
+        __syncwarp();
         if (seen) {
-          __syncwarp();
-          tc::load16(tmem + ((uint32_t)warp << 21) + S::kO + i, x);
+          tc::load8(mine + S::kO + i, x);
           tc::wait_load();
         }
-        if (live) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          f[e] = none ? 0.f : __uint_as_float(x[e]) * inv;
+        if (!live) continue;
+        if (a.splits == 1) {
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * a.o_row +
+                                    h * a.o_head + i) = Vec<T>::pack(f);
+        } else {
           float4* o = reinterpret_cast<float4*>(a.part + at * a.dim + i);
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            if (i + e >= a.dim) break;
-            float f[4];
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-              f[d] = none ? 0.f : __uint_as_float(x[e + d]) * inv;
-            o[e / 4] = make_float4(f[0], f[1], f[2], f[3]);
-          }
+          o[0] = make_float4(f[0], f[1], f[2], f[3]);
+          o[1] = make_float4(f[4], f[5], f[6], f[7]);
         }
       }
     }
   }
   if (nt > 0) {
-    if (!ok && a.error) *a.error = 1;
+    if (!ok) *a.error = 1;
+    __syncwarp();
     tc::fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 4) {
       tc::fence_after();
       tc::tmem_free(tmem, S::kColumns);
     }
@@ -348,14 +455,15 @@ __global__ void __launch_bounds__(128)
 }
 
 template <typename T, int kDim>
-cudaError_t launch(const CrossArgs& a, long long grid, cudaStream_t s) {
+cudaError_t launch(const CrossArgs& a, const Maps& maps, long long units,
+                   cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(
       cross_forward_kernel<T, kDim>,
       cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<kDim>::kSmem);
   if (e) return e;
   count_launches(1);
   cross_forward_kernel<T, kDim>
-      <<<(unsigned)grid, kThreads, Shape<kDim>::kSmem, s>>>(a);
+      <<<(unsigned)units, kThreads, Shape<kDim>::kSmem, s>>>(a, maps);
   if (a.splits > 1) {
     count_launches(1);
     cross_join_kernel<T>
@@ -363,8 +471,6 @@ cudaError_t launch(const CrossArgs& a, long long grid, cudaStream_t s) {
   }
   return cudaGetLastError();
 }
-
-int forward_keys(int dim) { return dim <= 64 ? 128 : 64; }
 
 }  // namespace
 
@@ -393,6 +499,51 @@ bool cross_sizes(const attention_args* a) {
          a->max_q <= a->n_q && a->max_k >= 0 && a->max_k <= a->n_k &&
          a->max_q * (a->heads / a->kv_heads) < kMaxInt - 2 * kRows &&
          a->max_k < kMaxInt - 2 * kRows;
+}
+
+namespace {
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
+                                void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion,
+                                CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static const EncodeTiled f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000,
+                                         cudaEnableDefault, &found) ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return f;
+}
+}  // namespace
+
+cudaError_t row_map(CUtensorMap* map, long long type, const feature_rows& t,
+                    long long dim, long long heads, long long rows,
+                    int heads_box, int rows_box) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return cudaErrorNotSupported;
+  const cuuint64_t size[3] = {(cuuint64_t)dim, (cuuint64_t)heads,
+                              (cuuint64_t)rows};
+  // a dimension of one element is never stepped along
+  const cuuint64_t step[2] = {
+      (cuuint64_t)(heads > 1 ? t.head * 2 : dim * 2),
+      (cuuint64_t)(rows > 1 ? t.row * 2 : heads * dim * 2)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)heads_box, (cuuint32_t)rows_box};
+  const cuuint32_t each[3] = {1, 1, 1};
+  const CUresult e = encode(
+      map,
+      type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+      3, const_cast<void*>(t.data), size, step, box, each,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return e == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 CrossArgs cross_arguments(const attention_args* in) {
@@ -440,7 +591,7 @@ ForwardPlan forward_plan(const attention_args* a) {
   ForwardPlan p;
   p.tiles = ceil_div(a->max_q * (a->heads / a->kv_heads), kRows);
   const long long blocks = p.tiles * a->scenes * a->kv_heads;
-  p.splits = split_count(blocks, ceil_div(a->max_k, forward_keys((int)a->dim)),
+  p.splits = split_count(blocks, ceil_div(a->max_k, kKeys),
                          2 * multiprocessors());
   p.blocks = blocks * p.splits;
   p.bytes =
@@ -477,10 +628,18 @@ GSA_API int cross_attention(const attention_args* in) {
   a.splits = p.splits;
   a.part = static_cast<float*>(in->workspace);
   if (p.splits > 1) a.part_lse = a.part + p.splits * a.n_q * a.heads * a.dim;
+  Maps maps = {};
+  if (in->n_k) {
+    cudaError_t e = row_map(&maps.k, in->type, in->k, a.dim, a.kv_heads, a.n_k,
+                            1, kKeys);
+    if (!e)
+      e = row_map(&maps.v, in->type, in->v, a.dim, a.kv_heads, a.n_k, 1, kKeys);
+    if (e) return e;
+  }
   cudaStream_t s = (cudaStream_t)in->stream;
   if (in->type == kF16)
-    return a.dim <= 64 ? launch<__half, 64>(a, p.blocks, s)
-                       : launch<__half, 128>(a, p.blocks, s);
-  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, p.blocks, s)
-                     : launch<__nv_bfloat16, 128>(a, p.blocks, s);
+    return a.dim <= 64 ? launch<__half, 64>(a, maps, p.blocks, s)
+                       : launch<__half, 128>(a, maps, p.blocks, s);
+  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, maps, p.blocks, s)
+                     : launch<__nv_bfloat16, 128>(a, maps, p.blocks, s);
 }

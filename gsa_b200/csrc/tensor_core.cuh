@@ -20,25 +20,40 @@ __device__ __forceinline__ void barrier_init(uint32_t bar, int count) {
                : "memory");
 }
 
-__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n"
-      " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+// Arrives and adds the bytes of the copies that the phase waits for.
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                   bar),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void barriers_ready() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 
-// Every wait is for products already issued, which take microseconds; the
-// limit (seconds) turns a fault of the program into an error.
+// Every wait is for work of the same block that is under way and takes
+// microseconds; the limit (seconds) turns a fault of the program into an
+// error.  The loop is written out so that the common case, a phase that is
+// complete, falls through (270 against 276 us of a forward pass).
 constexpr int kWaitLimit = 1 << 22;
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < kWaitLimit; ++i)
-    if (barrier_try(bar, parity)) return true;
-  return false;
+  uint32_t left;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+      "WAIT_AGAIN_%=:\n"
+      " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " @p bra WAIT_DONE_%=;\n"
+      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n"
+      " @q bra WAIT_AGAIN_%=;\n"
+      "WAIT_DONE_%=:\n mov.u32 %0, n;\n}\n"
+      : "=r"(left)
+      : "r"(bar), "r"(parity), "n"(kWaitLimit)
+      : "memory");
+  return left != 0;
 }
 
 // ---- tensor memory --------------------------------------------------------
@@ -99,6 +114,24 @@ __device__ __forceinline__ void load16(uint32_t at, uint32_t* r) {
         "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
         "=r"(r[15])
       : "r"(at));
+}
+
+__device__ __forceinline__ void load8(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]),
+        "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(at));
+}
+
+__device__ __forceinline__ void store8(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+      "r"(r[6]), "r"(r[7])
+      : "memory");
 }
 
 __device__ __forceinline__ void store16(uint32_t at, const uint32_t* r) {
@@ -173,34 +206,57 @@ __device__ __forceinline__ void commit(uint32_t bar) {
       : "memory");
 }
 
-// D[128][n] (+)= A[128][16 steps] B[n][16 steps]^T, both by columns; a and b
-// of `a_rows` and `b_rows` rows.
-template <typename T>
-__device__ __forceinline__ void product_by_columns(uint32_t d, uint32_t a,
-                                                   int a_rows, uint32_t b,
-                                                   int b_rows, int n,
-                                                   int steps) {
-  const uint32_t instr = instruction<T>(n, false);
-  for (int s = 0; s < steps; ++s) {
-    const uint32_t in = (s & 3) * 32;
-    mma(d, by_columns(a + (s >> 2) * a_rows * 128 + in),
-        by_columns(b + (s >> 2) * b_rows * 128 + in), instr, s > 0);
-  }
+// One lane of a converged warp.  Products are issued under it by warps that
+// run as one, so that their operands are known to be uniform: from a lone
+// thread each took 70 clocks to issue.
+__device__ __forceinline__ bool elect() {
+  uint32_t yes;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(yes));
+  return yes != 0;
 }
 
-// D[128][n] (+)= A[128][16 steps] B[16 steps][n], A in tensor memory, B's
-// tile of b_rows rows by rows.
-template <typename T>
+// D[128][n] (+)= A[128][16 steps] B[n][16 steps]^T, both by columns; a and b
+// of kA and kB rows, at most kSteps steps.
+template <typename T, int kA, int kB, int kSteps>
+__device__ __forceinline__ void product_by_columns(uint32_t d, uint32_t a,
+                                                   uint32_t b, int steps) {
+  const uint32_t instr = instruction<T>(kB, false);
+  const uint64_t a0 = by_columns(a), b0 = by_columns(b);
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+    if (s < steps)
+      mma(d, a0 + ((s >> 2) * kA * 128 + (s & 3) * 32) / 16,
+          b0 + ((s >> 2) * kB * 128 + (s & 3) * 32) / 16, instr, s > 0);
+}
+
+// D[128][n] (+)= A[128][kB] B[kB][n], A in tensor memory, B's tile of kB rows
+// by rows.
+template <typename T, int kB>
 __device__ __forceinline__ void product_by_rows(uint32_t d, uint32_t a,
-                                                uint32_t b, int b_rows, int n,
-                                                int steps, bool add) {
+                                                uint32_t b, int n, bool add) {
   const uint32_t instr = instruction<T>(n, true);
-  for (int s = 0; s < steps; ++s)
-    mma_tmem(d, a + s * 8, by_rows(b + s * 2048, b_rows * 128), instr,
-             add || s > 0);
+  const uint64_t b0 = by_rows(b, kB * 128);
+#pragma unroll
+  for (int s = 0; s < kB / 16; ++s)
+    mma_tmem(d, a + s * 8, b0 + s * 2048 / 16, instr, add || s > 0);
 }
 
 // ---- copies ---------------------------------------------------------------
+
+// A box of a tensor map (columns, head, row) into a panel of shared memory;
+// the barrier gets its bytes.  The column is a multiple of 64.
+__device__ __forceinline__ void copy_box(uint32_t to, const void* map,
+                                         uint32_t bar, int column, int head,
+                                         int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
+      "l"(map), "r"(bar), "r"(column), "r"(head), "r"(row)
+      : "memory");
+}
 
 // 16 bytes from global to shared memory, or zeros.
 __device__ __forceinline__ void copy16(uint32_t to, const void* from,
@@ -220,6 +276,32 @@ __device__ __forceinline__ void copy_wait() {
 // core (after the block's barrier).
 __device__ __forceinline__ void fence_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// ---- pairs of 32-bit values -------------------------------------------------
+
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float* lo, float* hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 }  // namespace tc
