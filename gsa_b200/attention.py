@@ -22,6 +22,7 @@ from ._library import current_stream
 
 MAX_DIM = 128
 MAX_WIDTH = 32
+MAX_GROUP = 64  # query heads per head of keys, cross attention
 _INT_MAX = (1 << 31) - 1
 
 
@@ -79,6 +80,8 @@ class _Call:
             raise ValueError("the head size must be a multiple of 8, at most 128")
         if not (self.kv_heads and self.heads and self.heads % self.kv_heads == 0):
             raise ValueError("the query heads must be a multiple of the keys' heads")
+        if types is _HALF and self.heads // self.kv_heads > MAX_GROUP:
+            raise ValueError("at most 64 query heads share a head of keys")
         if (n_q, n_k) != (pairs.n_q, pairs.n_k):
             raise ValueError("query and key rows must be those of the pairs' offsets")
         if scale is None:
@@ -180,8 +183,8 @@ def cross_attention(q, k, v, pairs, mask=None, scale=None, out=None, return_lse=
     scene.
 
     ``q``: BF16 or FP16 (N_q, heads, dim); ``k``, ``v``: the same type
-    (N_k, kv_heads, dim), heads a multiple of kv_heads (query head h reads
-    head h // (heads // kv_heads)); dim a multiple of 8, at most 128.  Row
+    (N_k, kv_heads, dim), heads a multiple of kv_heads, at most 64 times (query
+    head h reads head h // (heads // kv_heads)); dim a multiple of 8, at most 128.  Row
     and head strides are free in steps of 16 bytes.  ``mask``: bool (N_k,),
     False shuts a key out, whatever it holds.  ``scale``: dim ** -0.5 by
     default.  A query without open keys gets 0.  Returns ``out`` (written to

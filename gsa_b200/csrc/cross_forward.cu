@@ -495,7 +495,9 @@ int split_count(long long blocks, long long tiles, int room) {
 }
 
 bool cross_sizes(const attention_args* a) {
-  return attention_sizes(a) && a->type != kF32 && a->max_q >= 0 &&
+  // a box of packed rows holds at least one query row
+  return attention_sizes(a) && a->type != kF32 &&
+         a->heads / a->kv_heads <= 64 && a->max_q >= 0 &&
          a->max_q <= a->n_q && a->max_k >= 0 && a->max_k <= a->n_k &&
          a->max_q * (a->heads / a->kv_heads) < kMaxInt - 2 * kRows &&
          a->max_k < kMaxInt - 2 * kRows;
