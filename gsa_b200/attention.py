@@ -13,7 +13,6 @@ offsets of the query rows and of the key rows of every scene.
 """
 
 import itertools
-import math
 
 import torch
 
@@ -86,8 +85,8 @@ class _Call:
             raise ValueError("query and key rows must be those of the pairs' offsets")
         if scale is None:
             scale = self.dim ** -0.5
-        if not (math.isfinite(scale) and scale > 0):
-            raise ValueError("scale must be positive and finite")
+        if not 2.0**-24 <= scale <= 2.0**24:
+            raise ValueError("scale must be positive, from 2^-24 to 2^24")
         self.what, self.dtype, self.pairs, self.scale = what, q.dtype, pairs, scale
         self.q_shape, self.k_shape = q.shape, torch.Size((n_k, self.kv_heads, self.dim))
         self.rows = [self.rows_of(t, n, s) for t, n, s in (
@@ -187,7 +186,7 @@ def cross_attention(q, k, v, pairs, mask=None, scale=None, out=None, return_lse=
     head h reads head h // (heads // kv_heads)); dim a multiple of 8, at most 128.  Row
     and head strides are free in steps of 16 bytes.  ``mask``: bool (N_k,),
     False shuts a key out, whatever it holds.  ``scale``: dim ** -0.5 by
-    default.  A query without open keys gets 0.  Returns ``out`` (written to
+    default, from 2^-24 to 2^24.  A query without open keys gets 0.  Returns ``out`` (written to
     ``out`` if given), and with ``return_lse`` also the FP32 (N_q, heads)
     logarithms of the sums of exponentials that ``cross_attention_grad``
     takes.  Without ``out``, differentiable in q, k and v."""

@@ -15,8 +15,11 @@ struct CrossArgs {
   const void *q, *k, *v, *out, *dout;
   const unsigned char* mask;  // [n_k], 0 shuts a key out; may be null
   const int *q_seg, *k_seg;
-  float* lse;    // [n_q][heads], natural
-  float* delta;  // [n_q][heads]
+  float* lse;  // [n_q][heads], natural
+  // what the keys' pass needs of a packed row, [kv_heads][n_q * group]: its
+  // -lse in units of q k^T (less the factor that P carries) and its -delta, in
+  // three parts of the inputs' type each
+  uint4* row_values;
   void *o, *dq, *dk, *dv;
   float* part;      // [splits][rows][heads][dim] partial results
   float* part_lse;  // [splits][n_q][heads]
@@ -26,6 +29,7 @@ struct CrossArgs {
       d_head;
   int scenes, heads, kv_heads, group, dim, tiles, splits;
   float scale, scale_log2e;
+  int scale_exponent;  // 1 / scale is at most 2^this, where that is below 2^15
 };
 
 constexpr int kRows = 128;     // rows of a resident tile
@@ -70,24 +74,25 @@ __device__ __forceinline__ void load_packed(const Chunks& c, uint32_t tile,
 }
 
 // Zeros in the rows of a tile of kN rows whose bit is not set in `open` (a
-// word per 32 rows), by one warp.
+// word per 32 rows), by one warp: four rows at a time, 16 bytes a lane.  A
+// small loop: it runs once in a block's life, and its instructions come from
+// far.
 template <int kN>
 __device__ __forceinline__ void clear_rows(uint32_t tile, int panels,
                                            const uint32_t* open) {
   const int lane = threadIdx.x & 31;
+  tile += (lane >> 3) * 128 + (lane & 7) * 16;
 #pragma unroll
   for (int w = 0; w < kN / 32; ++w) {
-    uint32_t shut = ~open[w];
-    while (shut) {
-      const int row = w * 32 + __ffs(shut) - 1;
-      shut &= shut - 1;
-      if (lane < panels * 8)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                         tile + (lane >> 3) * kN * 128 + row * 128 +
-                         (lane & 7) * 16),
-                     "r"(0)
-                     : "memory");
-    }
+    uint32_t shut = ~open[w] >> (lane >> 3);
+#pragma unroll 1
+    for (int i = 0; shut; i += 4, shut >>= 4)
+      if (shut & 1)
+        for (int p = 0; p < panels; ++p)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                           tile + p * kN * 128 + (w * 32 + i) * 128),
+                       "r"(0)
+                       : "memory");
   }
 }
 

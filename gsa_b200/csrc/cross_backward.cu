@@ -15,43 +15,59 @@
 // products' left side; the walked tile serves as the right side of both its
 // products, read by columns and by rows, without a transposed copy.
 //
-// A block has eight warps of rows (two threads share a row, half of the walked
-// columns each), one that issues products, one that loads walked tiles (TMA;
-// rows behind the scene's last and shut keys are cleared).  The scores of the
-// next tile are taken as soon as this one's are in registers, so products run
-// beside the exponentials; P and dS have columns of their own.
+// A block has sixteen warps of rows (four threads share a row, a quarter of the
+// walked columns each), a warp for the products that give scores, one for the
+// others, which read what the rows make of them, and one that loads walked
+// tiles (TMA; rows behind the scene's last and shut keys are cleared).  The
+// scores of the next tile are taken as soon as this one's are in registers;
+// P and dS have columns of their own.
+//
+// In the keys' pass lse and delta belong to the columns.  They come from the
+// products themselves: 16 columns more, powers of two on the keys' side and on
+// the walked side -lse / scale and -delta in three parts of the inputs' type
+// (24 bits and more together), so that S and dP leave the tensor core less lse
+// and delta.  Read from shared memory (131 KB for 128 x 128 scores) they took
+// as long as all the exponentials.
 //
 // P and dS are rounded to the inputs' type for their products (half a step).
 // For fp16, whose smallest normal is 2^-14, P carries a factor of 2^15 (it is
 // at most 1) and dS one that grows with the number of keys.
 //
-// What bounds it, for 128 x 128 scores and a head of 64: 1,024 clocks of
-// products in the keys' pass (768 in the queries') beside 1,024 of
+// What bounds it, for 128 x 128 scores and a head of 64: 1,400 clocks of
+// products in the keys' pass (1,024 in the queries') beside 1,024 of
 // exponentials.
 #include "cross.cuh"
 
 namespace gsa {
 namespace {
 
-constexpr int kRowWarps = 8;
-constexpr int kBackThreads = 32 * (kRowWarps + 2);
 
 template <int kDim, bool kKeysPass>
 struct Shape {
-  // Rows of a walked tile: 128 where tensor memory has room for their scores.
-  static constexpr int kWalk = kDim == 128 && kKeysPass ? 64 : 128;
-  static constexpr int kStages = kDim == 128 && !kKeysPass ? 2 : 3;
-  static constexpr int kOwn = kRows * kDim * 2;    // bytes of a resident tile
-  static constexpr int kTile = kWalk * kDim * 2;   // of a walked one
-  static constexpr int kSmem = 1024 + 2 * kOwn + 2 * kStages * kTile;
-  static constexpr uint32_t kColumns = 512;
+  // The queries' pass of heads up to 64 fits an SM twice, with walked tiles of
+  // 64; the others walk 128 rows where tensor memory has room for their scores.
+  static constexpr int kBlocks = kDim == 64 && !kKeysPass ? 2 : 1;
+  static constexpr int kWalk =
+      kBlocks == 2 || (kDim == 128 && kKeysPass) ? 64 : 128;
+  static constexpr int kStages = kDim == 64 ? 4 : kKeysPass ? 3 : 2;
+  static constexpr int kRowWarps = kBlocks == 2 ? 8 : 16;
+  static constexpr int kShare = kRowWarps / 4;  // threads of a row
+  static constexpr int kThreads = 32 * (kRowWarps + 3);
+  static constexpr int kOwn = kRows * kDim * 2;   // bytes of a resident tile
+  static constexpr int kTile = kWalk * kDim * 2;  // of a walked one
+  // keys' pass: the further columns of a resident and of a walked tile
+  static constexpr int kOwnMore = kKeysPass ? kRows * 32 : 0;
+  static constexpr int kTileMore = kKeysPass ? kWalk * 32 : 0;
+  static constexpr int kSmem = 1024 + 2 * (kOwn + kOwnMore) +
+                               2 * kStages * (kTile + kTileMore);
+  static constexpr uint32_t kColumns = 512 / kBlocks;
   static constexpr uint32_t kS = 0, kDp = kWalk, kDs = 2 * kWalk;
   static constexpr uint32_t kP = kDs + kWalk / 2;  // keys' pass
   static constexpr uint32_t kOut1 = kKeysPass ? kP + kWalk / 2 : kP;
   static constexpr uint32_t kOut2 = kOut1 + kDim;  // keys' pass: dv
   static constexpr uint32_t kEnd = kKeysPass ? kOut2 + kDim : kOut2;
   static_assert(kEnd <= kColumns, "tensor memory");
-  static_assert(kSmem <= 225 * 1024, "shared memory");
+  static_assert(kBlocks * (kSmem + 4096) <= 227 * 1024, "shared memory");
 };
 
 struct BackMaps {
@@ -59,14 +75,14 @@ struct BackMaps {
 };
 
 enum Bar {
-  kTileFull = 0,    // [stage] a walked tile and its rows' values are there
-  kTileFree = 3,    // [stage] its products are complete
-  kTileRaw = 6,     // a tile loaded, rows to be cleared
-  kScores = 7,  // S and dP are complete
-  kRead = 8,    // S and dP are in registers (a count per warp of rows)
-  kWeights = 9,  // P and dS are there (a count per warp of rows)
-  kOutput = 10,  // the second products are complete
-  kBars = 11
+  kTileFull = 0,  // [stage] a walked tile is there
+  kTileFree = 4,  // [stage] its products are complete
+  kTileRaw = 8,   // a tile loaded, rows to be cleared
+  kScores = 9,    // S and dP are complete
+  kRead = 10,     // they are in registers (a count per warp)
+  kWeights = 11,  // P and dS are there (a count per warp)
+  kOutput = 12,   // the second products are complete
+  kBars = 13
 };
 
 // Factors that P and dS carry (2^x).
@@ -81,18 +97,42 @@ __device__ __forceinline__ float ds_bits(int keys) {
   return b > 0 ? (float)b : 0.f;
 }
 
+// x as three values of T that stand for multiples of 2^e, 2^(e-8) and
+// 2^(e-19): the exponents keep fp16 from overflowing (x below 2^(e+16)) and
+// from losing what lies below its normals.
+template <typename T>
+__device__ __forceinline__ uint2 three_parts(float x, int e) {
+  const float f0 = exp2f((float)e), f1 = exp2f((float)(e - 8)),
+              f2 = exp2f((float)(e - 19));
+  const float h = to_float(from_float<T>(x / f0));
+  float m = 0.f, l = 0.f;
+  if (fabsf(h) < kInf) {
+    const float r = x - h * f0;
+    m = to_float(from_float<T>(r / f1));
+    l = (r - m * f1) / f2;
+  }
+  return make_uint2(pack2<T>(h, m), pack2<T>(l, 0.f));
+}
+
+// The last 16 columns of a product by columns, from narrow tiles.
+template <typename T, int kN>
+__device__ __forceinline__ void product_more(uint32_t d, uint32_t a,
+                                             uint32_t b) {
+  tc::mma(d, tc::by_columns_narrow(a), tc::by_columns_narrow(b),
+          tc::instruction<T>(kN, false), true);
+}
+
 template <typename T, int kDim, bool kKeysPass>
-__global__ void __launch_bounds__(kBackThreads, 1)
+__global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
+                                  Shape<kDim, kKeysPass>::kBlocks)
     cross_backward_kernel(const __grid_constant__ CrossArgs a,
                           const __grid_constant__ BackMaps maps) {
   using S = Shape<kDim, kKeysPass>;
-  constexpr int W = S::kWalk;
+  constexpr int W = S::kWalk, kRowWarps = S::kRowWarps;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[kBars];
   __shared__ uint32_t tmem_at;
-  // -lse (base 2, less the factor that P carries) and -delta of the walked rows
-  __shared__ __align__(16) float row_lse[S::kStages][W];
-  __shared__ __align__(16) float row_delta[S::kStages][W];
+  __shared__ float part_delta[S::kShare][kRows];
 
   unsigned unit = blockIdx.x;
   const int r0 = unit % a.tiles * kRows;
@@ -116,6 +156,10 @@ __global__ void __launch_bounds__(kBackThreads, 1)
   const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
   const uint32_t x1 = smem, x2 = smem + S::kOwn, y1 = x2 + S::kOwn,
                  y2 = y1 + S::kStages * S::kTile;
+  const uint32_t x1_more = y2 + S::kStages * S::kTile,
+                 x2_more = x1_more + S::kOwnMore,
+                 y1_more = x2_more + S::kOwnMore,
+                 y2_more = y1_more + S::kStages * S::kTileMore;
   const uint32_t bar0 = tc::smem_address(bars);
   const int steps = (a.dim + 15) / 16;
   const unsigned char* mask = a.mask ? a.mask + k0 : nullptr;
@@ -125,15 +169,25 @@ __global__ void __launch_bounds__(kBackThreads, 1)
   auto wait = [&](int which, int phase) {
     if (ok) ok = tc::barrier_wait(bar0 + which * 8, phase & 1);
   };
+  auto store = [&](uint32_t at, uint32_t u0, uint32_t u1) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %3};" ::"r"(at), "r"(u0),
+                 "r"(u1), "r"(0)
+                 : "memory");
+  };
   const float bits = ds_bits<T>(nk);
   const float ds_factor = exp2f(bits - p_bits<T>());
+  // the exponents of the further columns' first part: of lse / scale, so that
+  // lse is below 2^16; of delta
+  const int s_exp = a.scale_exponent, d_exp = 8;
 
   if (nt > 0) {
     if (warp == kRowWarps) {
       tc::tmem_alloc(tc::smem_address(&tmem_at), S::kColumns);
       if (lane == 0) {
         for (int i = 0; i < kBars; ++i)
-          tc::barrier_init(bar(i), i == kRead || i == kWeights ? kRowWarps : 1);
+          tc::barrier_init(bar(i), i == kRead || i == kWeights ? kRowWarps
+                                   : kKeysPass && i < kTileFree ? 2
+                                                                : 1);
         tc::barriers_ready();
       }
       __syncwarp();
@@ -148,11 +202,41 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         for (int i = each * 8 + tid; i < W * 8; i += kRowWarps * 32)
           for (int s = 0; s < 2 * S::kStages; ++s)
             for (int p = 0; p < kDim / 64; ++p)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                               y1 + s * S::kTile + p * W * 128 + i * 16),
-                           "r"(0)
-                           : "memory");
+              store(y1 + s * S::kTile + p * W * 128 + i * 16, 0, 0);
+        // the resident tiles' further columns, and the second half (zeros) of
+        // the walked ones'
+        if (tid < kRows) {
+          for (int x = 0; x < 2; ++x) {
+            const int e = x ? d_exp : s_exp;
+            const uint32_t to = x ? x2_more : x1_more;
+            store(to + tc::narrow_offset(tid, 0),
+                  pack2<T>(exp2f((float)e), exp2f((float)(e - 8))),
+                  pack2<T>(exp2f((float)(e - 19)), 0.f));
+            store(to + tc::narrow_offset(tid, 1), 0, 0);
+          }
+        }
+        if (tid < W)
+          for (int s = 0; s < 2 * S::kStages; ++s)
+            store(y1_more + s * S::kTileMore + tc::narrow_offset(tid, 1), 0, 0);
       } else {
+        // delta = <dout, out>, a share of the row's elements each
+        const int r = min(r0 + (tid & (kRows - 1)), n - 1), qr = r / a.group;
+        const int h = hk * a.group + r - qr * a.group;
+        const T* o = static_cast<const T*>(a.out) + (q0 + qr) * a.o_row +
+                     h * a.o_head;
+        const T* d = static_cast<const T*>(a.dout) + (q0 + qr) * a.d_row +
+                     h * a.d_head;
+        constexpr int kEach = kDim / 8 / S::kShare;
+        uint4 u[kEach], v[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int at = ((tid >> 7) + i * S::kShare) * 8;
+          u[i] = v[i] = make_uint4(0, 0, 0, 0);
+          if (at < a.dim) {
+            u[i] = *reinterpret_cast<const uint4*>(o + at);
+            v[i] = *reinterpret_cast<const uint4*>(d + at);
+          }
+        }
         const long long head = (long long)hk * a.group;
         load_packed<T, kRows>(
             c, x1, static_cast<const T*>(a.q) + q0 * a.q_row + head * a.q_head,
@@ -161,6 +245,16 @@ __global__ void __launch_bounds__(kBackThreads, 1)
             c, x2,
             static_cast<const T*>(a.dout) + q0 * a.d_row + head * a.d_head,
             a.d_row, a.d_head, a.group, r0, n);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          float x[8], y[8];
+          Vec<T>::unpack(u[i], x);
+          Vec<T>::unpack(v[i], y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
+        }
+        part_delta[tid >> 7][tid & (kRows - 1)] = sum;
       }
       tc::copy_commit();
       tc::copy_wait<0>();
@@ -175,99 +269,102 @@ __global__ void __launch_bounds__(kBackThreads, 1)
   if (warp == kRowWarps + 1) {
     const int panels = a.dim > 64 ? 2 : 1;
     int cleared = 0;
+    // the values of the next tile's rows are on their way while this one's
+    // place is waited for
+    uint4 values[W / 32];
+    const uint4 nothing =  // lse = inf: P = 0
+        make_uint4(pack2<T>(-kInf, 0.f), 0, 0, 0);
+    auto load_values = [&](int t) {
+      const int first = (begin + t) * each;
+      const long long at = ((long long)hk * a.n_q + q0) * a.group;
+#pragma unroll
+      for (int i = 0; i < W / 32; ++i) {
+        const int r = first + i * 32 + lane;
+        const bool there = t < nt && i * 32 + lane < each && r < n;
+        values[i] = there ? a.row_values[at + r] : nothing;
+      }
+    };
+    if constexpr (kKeysPass) load_values(0);
     for (int t = 0; t < nt; ++t) {
       const int stage = t % S::kStages;
       const int at = (begin + t) * each;
       const uint32_t t1 = y1 + stage * S::kTile, t2 = y2 + stage * S::kTile;
       uint32_t open[W / 32];
-      bool whole = true;
+      bool whole;
       if constexpr (kKeysPass) {
         key_words<W>(open, nullptr, 0, min(n - at, each));
         whole = n - at >= each;
       } else {
         key_words<W>(open, mask, at, nk);
+        whole = true;
 #pragma unroll
         for (int i = 0; i < W / 32; ++i) whole &= open[i] == 0xffffffffu;
       }
-      float lse[W / 32], delta[W / 32];
-      if constexpr (kKeysPass) {
-#pragma unroll
-        for (int i = 0; i < W / 32; ++i) {
-          const int r = at + i * 32 + lane;
-          lse[i] = -kInf;  // P = 0: an absent row, or one without keys
-          delta[i] = 0.f;
-          if (i * 32 + lane < each && r < n) {
-            const int qr = r / a.group;
-            const long long e = (long long)(q0 + qr) * a.heads +
-                                hk * a.group + (r - qr * a.group);
-            const float x = __ldg(a.lse + e);
-            if (x != -kInf) lse[i] = fmaf(x, -kLog2e, p_bits<T>());
-            delta[i] = -a.delta[e] * ds_factor;
-          }
-        }
-      }
       if (t >= S::kStages) wait(kTileFree + stage, t / S::kStages - 1);
-      if constexpr (kKeysPass) {
-#pragma unroll
-        for (int i = 0; i < W / 32; ++i) {
-          row_lse[stage][i * 32 + lane] = lse[i];
-          row_delta[stage][i * 32 + lane] = delta[i];
-        }
-      }
       const int full = whole ? kTileFull + stage : kTileRaw;
       __syncwarp();
       if (tc::elect()) {
         tc::barrier_expect(bar(full), 2 * panels * each * 128);
+        const int head = kKeysPass ? hk * a.group : hk;
+        const int row = kKeysPass ? q0 + at / a.group : k0 + at;
         for (int p = 0; p < panels; ++p) {
-          if constexpr (kKeysPass) {
-            const int head = hk * a.group, row = q0 + at / a.group;
-            tc::copy_box(t1 + p * W * 128, &maps.y1, bar(full), p * 64, head,
-                         row);
-            tc::copy_box(t2 + p * W * 128, &maps.y2, bar(full), p * 64, head,
-                         row);
-          } else {
-            tc::copy_box(t1 + p * W * 128, &maps.y1, bar(full), p * 64, hk,
-                         k0 + at);
-            tc::copy_box(t2 + p * W * 128, &maps.y2, bar(full), p * 64, hk,
-                         k0 + at);
-          }
+          tc::copy_box(t1 + p * W * 128, &maps.y1, bar(full), p * 64, head,
+                       row);
+          tc::copy_box(t2 + p * W * 128, &maps.y2, bar(full), p * 64, head,
+                       row);
         }
+      }
+      if constexpr (kKeysPass) {
+#pragma unroll
+        for (int i = 0; i < W / 32; ++i) {
+          const uint32_t to =
+              stage * S::kTileMore + tc::narrow_offset(i * 32 + lane, 0);
+          store(y1_more + to, values[i].x, values[i].y);
+          store(y2_more + to, values[i].z, values[i].w);
+        }
+        load_values(t + 1);
       }
       if (!whole) {
         wait(kTileRaw, cleared++);
         __syncwarp();
         clear_rows<W>(t1, panels, open);
-        clear_rows<W>(t2, panels, open);
+        if constexpr (kKeysPass) clear_rows<W>(t2, panels, open);
+      }
+      if (!whole || kKeysPass) {
         tc::fence_shared();
         __syncwarp();
-        if (lane == 0) tc::barrier_arrive(bar(kTileFull + stage));
+        // in the keys' pass a tile is there with its copies and its values
+        if (lane == 0) {
+          tc::barrier_arrive(bar(kTileFull + stage));
+          if (!whole && kKeysPass) tc::barrier_arrive(bar(kTileFull + stage));
+        }
       }
     }
   } else if (warp == kRowWarps) {
-    auto scores = [&](int t) {
+    for (int t = 0; t < nt; ++t) {
       const int stage = t % S::kStages;
+      wait(kTileFull + stage, t / S::kStages);
+      if (t > 0) wait(kRead, t - 1);
       tc::fence_after();
       __syncwarp();
       if (tc::elect()) {
         tc::product_by_columns<T, kRows, W, kDim / 16>(
             tmem + S::kS, x1, y1 + stage * S::kTile, steps);
+        if constexpr (kKeysPass)
+          product_more<T, W>(tmem + S::kS, x1_more,
+                             y1_more + stage * S::kTileMore);
         tc::product_by_columns<T, kRows, W, kDim / 16>(
             tmem + S::kDp, x2, y2 + stage * S::kTile, steps);
+        if constexpr (kKeysPass)
+          product_more<T, W>(tmem + S::kDp, x2_more,
+                             y2_more + stage * S::kTileMore);
         tc::commit(bar(kScores));
       }
       __syncwarp();
-    };
-    if (nt > 0) {
-      wait(kTileFull, 0);
-      scores(0);
     }
+  } else if (warp == kRowWarps + 2) {
     for (int t = 0; t < nt; ++t) {
       const int stage = t % S::kStages;
-      if (t + 1 < nt) {
-        wait(kTileFull + (t + 1) % S::kStages, (t + 1) / S::kStages);
-        wait(kRead, t);
-        scores(t + 1);
-      }
       wait(kWeights, t);
       tc::fence_after();
       __syncwarp();
@@ -283,10 +380,9 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       __syncwarp();
     }
   } else {
-    constexpr int kMine = W / 2;  // a thread's columns of its row
-    const int half = warp >> 2, group = warp & 3;
-    const int in_tile = group * 32 + lane;
-    const int r = r0 + in_tile;
+    constexpr int kMine = W / S::kShare;  // a thread's columns of its row
+    const int part = warp >> 2, group = warp & 3;
+    const int r = r0 + group * 32 + lane;
     const bool live = r < own;
     const bool busy = r0 + group * 32 < own;  // the warp holds rows
     const uint32_t mine = tmem + ((uint32_t)group << 21);
@@ -295,25 +391,22 @@ __global__ void __launch_bounds__(kBackThreads, 1)
     if constexpr (kKeysPass) {
       open = live && (!mask || __ldg(mask + r));
     } else if (nt > 0) {
-      const int qr = live ? r / a.group : 0;
-      const int h = hk * a.group + (live ? r - qr * a.group : 0);
-      const long long row = q0 + qr;
-      if (live) {
-        const T* o = static_cast<const T*>(a.out) + row * a.o_row +
-                     h * a.o_head;
-        const T* d = static_cast<const T*>(a.dout) + row * a.d_row +
-                     h * a.d_head;
-        for (int i = 0; i < a.dim; i += 8) {
-          float x[8], y[8];
-          Vec<T>::unpack(*reinterpret_cast<const uint4*>(o + i), x);
-          Vec<T>::unpack(*reinterpret_cast<const uint4*>(d + i), y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) delta = fmaf(x[e], y[e], delta);
-        }
-        const long long e = row * a.heads + h;
-        if (half == 0) a.delta[e] = delta;
-        const float x = __ldg(a.lse + e);
+      for (int i = 0; i < S::kShare; ++i)
+        delta += part_delta[i][group * 32 + lane];
+      if (live) {
+        const int qr = r / a.group;
+        const long long row = q0 + qr;
+        const int h = hk * a.group + (r - qr * a.group);
+        // a row without keys gets P = 0
+        const float x = __ldg(a.lse + row * a.heads + h);
         if (x != -kInf) lse2 = fmaf(x, -kLog2e, p_bits<T>());
+        if (part == 0) {
+          const long long e = ((long long)hk * a.n_q + q0) * a.group + r;
+          const uint2 u = three_parts<T>(lse2 / a.scale_log2e, s_exp);
+          const uint2 v = three_parts<T>(-delta, d_exp);
+          a.row_values[e] = make_uint4(u.x, u.y, v.x, v.y);
+        }
       }
       delta *= -ds_factor;
     }
@@ -321,6 +414,8 @@ __global__ void __launch_bounds__(kBackThreads, 1)
     const bool all_open = __all_sync(kFull, open);
     const uint64_t scale2 = tc::pair(a.scale_log2e, a.scale_log2e);
     const uint64_t factor2 = tc::pair(ds_factor, ds_factor);
+    const uint64_t row_lse2 = tc::pair(lse2, lse2);
+    const uint64_t row_delta2 = tc::pair(delta, delta);
     if (!busy) {
       for (int t = 0; t < nt; ++t) {
         wait(kScores, t);
@@ -331,95 +426,81 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         __syncwarp();
       }
     } else {
+      const uint32_t at = mine + part * kMine;
+      const uint32_t to = mine + part * (kMine / 2);
       for (int t = 0; t < nt; ++t) {
-        const int stage = t % S::kStages;
         uint32_t s[kMine], d[kMine];
-        if constexpr (kKeysPass) wait(kTileFull + stage, t / S::kStages);
         wait(kScores, t);
         __syncwarp();
         tc::fence_after();
-#pragma unroll
-        for (int i = 0; i < kMine; i += 32) {
-          tc::load32(mine + S::kS + half * kMine + i, s + i);
-          tc::load32(mine + S::kDp + half * kMine + i, d + i);
+        if constexpr (kMine == 32) {
+          tc::load32(at + S::kS, s);
+          tc::load32(at + S::kDp, d);
+        } else {
+          tc::load16(at + S::kS, s);
+          tc::load16(at + S::kDp, d);
         }
         tc::wait_load();
         tc::fence_before();
         __syncwarp();
         if (lane == 0) tc::barrier_arrive(bar(kRead));
-        bool whole = true;
-        uint32_t words[W / 32];
-        if constexpr (!kKeysPass) {
-          const int at = (begin + t) * W;
-          if (mask || at + W > nk) {
-            key_words<W>(words, mask, at, nk);
-            whole = false;
-          }
-        } else {
-          whole = all_open;
-        }
         uint32_t p[kMine / 2], ds[kMine / 2];
 #pragma unroll
-        for (int i = 0; i < kMine; i += 4) {
-          uint64_t l[2], e[2];
+        for (int i = 0; i < kMine; i += 2) {
+          uint64_t x = tc::pair(__uint_as_float(s[i]),
+                                __uint_as_float(s[i + 1]));
+          uint64_t e = tc::pair(__uint_as_float(d[i]),
+                                __uint_as_float(d[i + 1]));
           if constexpr (kKeysPass) {
-            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(
-                &row_lse[stage][half * kMine + i]);
-            const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(
-                &row_delta[stage][half * kMine + i]);
-            l[0] = x.x;
-            l[1] = x.y;
-            e[0] = y.x;
-            e[1] = y.y;
+            x = tc::mul2(x, scale2);
+            if constexpr (__is_same(T, __half)) e = tc::mul2(e, factor2);
           } else {
-            l[0] = l[1] = tc::pair(lse2, lse2);
-            e[0] = e[1] = tc::pair(delta, delta);
+            x = tc::fma2(x, scale2, row_lse2);
+            e = tc::fma2(e, factor2, row_delta2);
           }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int c = i + 2 * j;
-            float u0, u1, w0, w1;
-            tc::unpair(tc::fma2(tc::pair(__uint_as_float(s[c]),
-                                         __uint_as_float(s[c + 1])),
-                                scale2, l[j]), &u0, &u1);
-            u0 = exp2_fast(u0);
-            u1 = exp2_fast(u1);
-            tc::unpair(
-                tc::mul2(tc::pair(u0, u1),
-                         tc::fma2(tc::pair(__uint_as_float(d[c]),
-                                           __uint_as_float(d[c + 1])),
-                                  factor2, e[j])),
-                &w0, &w1);
-            if constexpr (kKeysPass) p[c / 2] = pack2<T>(u0, u1);
-            ds[c / 2] = pack2<T>(w0, w1);
-          }
+          float u0, u1, w0, w1;
+          tc::unpair(x, &u0, &u1);
+          u0 = exp2_fast(u0);
+          u1 = exp2_fast(u1);
+          tc::unpair(tc::mul2(tc::pair(u0, u1), e), &w0, &w1);
+          if constexpr (kKeysPass) p[i / 2] = pack2<T>(u0, u1);
+          ds[i / 2] = pack2<T>(w0, w1);
         }
-        if (!whole) {
+        if constexpr (kKeysPass) {
+          if (!all_open) {
 #pragma unroll
-          for (int i = 0; i < kMine / 2; ++i) {
-            uint32_t keep;
-            if constexpr (kKeysPass) {
-              keep = open ? 0xffffffffu : 0u;
-              p[i] &= keep;
-            } else {
-              const uint32_t word =
-                  half ? words[W / 64 + i / 16] : words[i / 16];
-              const uint32_t two = word >> ((2 * i) & 31);
-              keep = ((two & 1) ? 0xffffu : 0u) |
-                     ((two & 2) ? 0xffff0000u : 0u);
+            for (int i = 0; i < kMine / 2; ++i) {
+              p[i] = open ? p[i] : 0u;
+              ds[i] = open ? ds[i] : 0u;
             }
-            ds[i] &= keep;
+          }
+        } else {
+          const int first = (begin + t) * W;
+          if (mask || first + W > nk) {
+            uint32_t words[W / 32];
+            key_words<W>(words, mask, first, nk);
+            uint32_t word = words[0];  // of this thread's 32 columns
+#pragma unroll
+            for (int i = 1; i < W / 32; ++i)
+              if (part == i) word = words[i];
+#pragma unroll
+            for (int i = 0; i < kMine / 2; ++i) {
+              const uint32_t two = word >> (2 * i);
+              ds[i] &= ((two & 1) ? 0xffffu : 0u) |
+                       ((two & 2) ? 0xffff0000u : 0u);
+            }
           }
         }
         // P's and dS's places are free once the last products are complete
         if (t > 0) wait(kOutput, t - 1);
         __syncwarp();
         tc::fence_after();
-#pragma unroll
-        for (int i = 0; i < kMine / 2; i += 16) {
-          if constexpr (kKeysPass)
-            tc::store16(mine + S::kP + half * (kMine / 2) + i, p + i);
-          tc::store16(mine + S::kDs + half * (kMine / 2) + i, ds + i);
+        if constexpr (kMine == 32) {
+          if constexpr (kKeysPass) tc::store16(to + S::kP, p);
+          tc::store16(to + S::kDs, ds);
+        } else {
+          if constexpr (kKeysPass) tc::store8(to + S::kP, p);
+          tc::store8(to + S::kDs, ds);
         }
         tc::wait_store();
         tc::fence_before();
@@ -450,9 +531,8 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       for (int which = 0; which < (kKeysPass ? 2 : 1); ++which) {
         const float f = which ? exp2f(-p_bits<T>()) : a.scale * exp2f(-bits);
         T* out = static_cast<T*>(kKeysPass ? (which ? a.dv : a.dk) : a.dq) + at;
-        float* part =
-            a.part + ((kKeysPass ? 2 : 1) * split + which) * parts + at;
-        for (int i = half * 8; i < a.dim; i += 16) {
+        float* sum = a.part + ((kKeysPass ? 2 : 1) * split + which) * parts + at;
+        for (int i = part * 8; i < a.dim; i += 8 * S::kShare) {
           uint32_t x[8];
           float y[8];
           __syncwarp();
@@ -467,7 +547,7 @@ __global__ void __launch_bounds__(kBackThreads, 1)
           if (a.splits == 1) {
             *reinterpret_cast<uint4*>(out + i) = Vec<T>::pack(y);
           } else {
-            float4* o = reinterpret_cast<float4*>(part + i);
+            float4* o = reinterpret_cast<float4*>(sum + i);
             o[0] = make_float4(y[0], y[1], y[2], y[3]);
             o[1] = make_float4(y[4], y[5], y[6], y[7]);
           }
@@ -509,23 +589,26 @@ __global__ void __launch_bounds__(256)
 struct Plan {
   long long tiles[2], blocks[2];  // of the keys' pass, of the queries'
   int splits[2];
-  long long delta, part;  // bytes
+  long long values, part;  // bytes
 };
 
 Plan backward_plan(const attention_args* a) {
   Plan p;
   const long long rows = a->max_q * (a->heads / a->kv_heads);
-  const int room = multiprocessors();
   p.tiles[0] = ceil_div(a->max_k, kRows);
   p.tiles[1] = ceil_div(rows, kRows);
-  const long long walked[2] = {ceil_div(rows, a->dim <= 64 ? 128 : 64),
-                               ceil_div(a->max_k, 128)};
+  const long long walked[2] = {
+      ceil_div(rows, a->dim <= 64 ? Shape<64, true>::kWalk
+                                  : Shape<128, true>::kWalk),
+      ceil_div(a->max_k, a->dim <= 64 ? Shape<64, false>::kWalk
+                                      : Shape<128, false>::kWalk)};
   for (int i = 0; i < 2; ++i) {
+    const int room = multiprocessors() * (i && a->dim <= 64 ? 2 : 1);
     p.blocks[i] = p.tiles[i] * a->scenes * a->kv_heads;
     p.splits[i] = split_count(p.blocks[i], walked[i], room);
     p.blocks[i] *= p.splits[i];
   }
-  p.delta = (a->n_q * a->heads * 4 + 15) / 16 * 16;
+  p.values = 16 * a->n_q * a->heads;
   // the two passes' parts follow one another in the same place
   const long long keys =
       p.splits[0] == 1 ? 0
@@ -566,7 +649,7 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
   if (e) return e;
   count_launches(1);
   cross_backward_kernel<T, kDim, kKeysPass>
-      <<<(unsigned)grid, kBackThreads, S::kSmem, s>>>(a, maps);
+      <<<(unsigned)grid, S::kThreads, S::kSmem, s>>>(a, maps);
   if (a.splits > 1) {
     const long long n =
         kKeysPass ? a.n_k * a.kv_heads * a.dim : a.n_q * a.heads * a.dim;
@@ -585,7 +668,7 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
   return cudaGetLastError();
 }
 
-// The queries' pass first: it leaves delta to the keys'.
+// The queries' pass first: it leaves its rows' lse and delta to the keys'.
 template <typename T>
 cudaError_t launch(const CrossArgs& a, const attention_args* in, const Plan& p,
                    cudaStream_t s) {
@@ -605,7 +688,7 @@ using namespace gsa;
 GSA_API int64_t cross_attention_grad_workspace(const attention_args* in) {
   if (!cross_sizes(in)) return -2;
   const Plan p = backward_plan(in);
-  return p.delta + p.part;
+  return p.values + p.part;
 }
 
 // See include/point_features.h.
@@ -623,17 +706,17 @@ GSA_API int cross_attention_grad(const attention_args* in) {
     return -2;
   const Plan p = backward_plan(in);
   if (p.blocks[0] > kMaxInt || p.blocks[1] > kMaxInt) return -2;
-  if (p.delta + p.part && (!vector_address(in->workspace) ||
-                           in->workspace_bytes < p.delta + p.part))
+  if (p.values + p.part && (!vector_address(in->workspace) ||
+                           in->workspace_bytes < p.values + p.part))
     return -2;
   CrossArgs a = cross_arguments(in);
   a.out = in->out.data;
   a.dout = in->dout.data;
   a.d_row = in->dout.row;
   a.d_head = in->dout.head;
-  a.delta = static_cast<float*>(in->workspace);
+  a.row_values = static_cast<uint4*>(in->workspace);
   a.part = reinterpret_cast<float*>(static_cast<char*>(in->workspace) +
-                                    p.delta);
+                                    p.values);
   a.dq = in->dq;
   a.dk = in->dk;
   a.dv = in->dv;

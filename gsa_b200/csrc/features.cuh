@@ -145,7 +145,7 @@ inline bool attention_sizes(const attention_args* a) {
          a->n_k * a->kv_heads / 4 < kMaxInt;
 }
 inline bool attention_scale(double scale) {
-  return scale > 0. && (float)scale > 0.f && (float)scale < kInf;
+  return scale >= 1. / (1 << 24) && scale <= (double)(1 << 24);
 }
 
 }  // namespace gsa

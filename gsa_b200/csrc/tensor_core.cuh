@@ -171,6 +171,16 @@ __device__ __forceinline__ uint64_t by_rows(uint32_t tile, uint32_t panel) {
          ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32);
 }
 
+// A tile of 16 columns without swizzle, summed over its columns: per 8 rows
+// their first 16 bytes, then their second.
+__device__ __forceinline__ uint32_t narrow_offset(int row, int chunk) {
+  return (uint32_t)((row >> 3) * 256 + chunk * 128 + (row & 7) * 16);
+}
+__device__ __forceinline__ uint64_t by_columns_narrow(uint32_t tile) {
+  return (1ull << 46) | ((tile >> 4) & 0x3fffu) |
+         ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(256 >> 4) << 32);
+}
+
 // Instruction: 128 x n products of fp16 or bf16 pairs summed in 32 bits.
 template <typename T>
 __device__ __forceinline__ uint32_t instruction(int n, bool b_by_rows) {

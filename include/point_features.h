@@ -63,7 +63,7 @@ typedef struct {
   int64_t heads, kv_heads;  /* heads a multiple of kv_heads: head h reads
                                head h / (heads / kv_heads) of the keys */
   int64_t dim;              /* a multiple of 8, at most 128 */
-  double scale;             /* positive */
+  double scale;             /* 2^-24 to 2^24 */
   feature_rows q, k, v;
   feature_rows out;         /* written forward, read backward */
   feature_rows dout;
