@@ -16,12 +16,14 @@
 // over all (row, entry) that name the key: the entries are sorted by key
 // first (stable), so the sums have one fixed order and need no atomics.
 //
-// The bound is the gather: every entry reads a key's and a value's head
-// through L2, D elements each, some tens of times what the tensors hold.  So
-// a head is a group of lanes with a 16-byte vector each, eight entries' loads
-// are in flight per group, and scores, softmax and sums stay in 32-bit
-// registers.
+// The bound is the gather and what each gathered element costs: an entry reads
+// a key's and a value's head through L2, and its elements are unpacked,
+// multiplied and added in 32 bits.  So nothing is done twice: a block first
+// lists the entries that count of its rows (once for all heads) in shared
+// memory; a head is a group of lanes with a 16-byte vector each, with several
+// entries' loads in flight, multiplying pairs at a time.
 #include "features.cuh"
+#include "tensor_core.cuh"
 
 namespace gsa {
 namespace {
@@ -43,7 +45,10 @@ struct NeighborArgs {
 };
 
 constexpr int kBlock = 128;
-constexpr int kAhead = 8;  // entries whose loads are in flight
+// Entries of a group whose loads are in flight: with 8 (or 2) the forward pass
+// of 192,000 rows takes 654 (549) us instead of 514.
+constexpr int kAhead = 4;
+constexpr int kListStride = 36;    // of a row's list, clear of bank conflicts
 
 template <int L>
 __device__ __forceinline__ float group_sum(float x) {
@@ -52,199 +57,232 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ float dot(const uint4& a, const float* b) {
-  float f[V], s = 0.f;
-  Vec<T>::unpack(a, f);
+// A vector's elements as pairs of 32-bit values.
+template <typename T>
+struct Pairs {
+  static constexpr int N = Vec<T>::V / 2;
+  uint64_t v[N];
+  __device__ __forceinline__ Pairs() {}
+  __device__ __forceinline__ explicit Pairs(const uint4& u) {
+    float f[2 * N];
+    Vec<T>::unpack(u, f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) s = fmaf(f[i], b[i], s);
-  return s;
-}
-
-// The keys that entries j0 .. j0 + kAhead of a row name (global key rows), or
-// -1 where an entry is absent.
-__device__ __forceinline__ void entries(const NeighborArgs& a, const int* ids,
-                                        int j0, int first, int base, int n,
-                                        int* at) {
-#pragma unroll
-  for (int t = 0; t < kAhead; ++t) {
-    const int j = j0 + t;
-    int id = j < a.width ? __ldg(ids + j) : -1;
-    if (a.padded && j > 0 && id == first) id = -1;
-    at[t] = (unsigned)id < (unsigned)n ? base + id : -1;
+    for (int i = 0; i < N; ++i) v[i] = tc::pair(f[2 * i], f[2 * i + 1]);
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0;
+  }
+  __device__ __forceinline__ float dot(const Pairs& o) const {
+    uint64_t s = tc::mul2(v[0], o.v[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) s = tc::fma2(v[i], o.v[i], s);
+    float a, b;
+    tc::unpair(s, &a, &b);
+    return a + b;
+  }
+  // this += w * o
+  __device__ __forceinline__ void add(float w, const Pairs& o) {
+    const uint64_t w2 = tc::pair(w, w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = tc::fma2(w2, o.v[i], v[i]);
+  }
+  __device__ __forceinline__ void scale(float w) {
+    const uint64_t w2 = tc::pair(w, w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = tc::mul2(v[i], w2);
+  }
+  __device__ __forceinline__ uint4 pack() const {
+    float f[2 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) tc::unpair(v[i], &f[2 * i], &f[2 * i + 1]);
+    return Vec<T>::pack(f);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 vector_at(const void* base, long long element) {
+  return __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) +
+                                              element));
 }
 
-// One group of L lanes per (row, head).
+// The block's rows from `first` on: the keys (global rows) that a row's
+// entries name, those that count, in their order; behind the last, the first
+// again up to a multiple of kAhead.
+template <int kRowsMax>
+struct RowLists {
+  int keys[kRowsMax][kListStride];
+  int count[kRowsMax];
+
+  __device__ __forceinline__ void fill(const NeighborArgs& a, long long first,
+                                       int rows) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = warp; i < rows; i += kBlock / 32) {
+      const long long row = first + i;
+      const int scene = scene_of(a.q_seg, a.scenes, (int)row);
+      const int base = __ldg(a.k_seg + scene);
+      const int n = __ldg(a.k_seg + scene + 1) - base;
+      const int id = lane < a.width ? __ldg(a.ids + row * a.width + lane) : -1;
+      const int head = __shfl_sync(kFull, id, 0);
+      const bool there = (unsigned)id < (unsigned)n &&
+                         !(a.padded && lane > 0 && id == head);
+      const unsigned set = __ballot_sync(kFull, there);
+      const int total = __popc(set);
+      if (there) keys[i][__popc(set & ((1u << lane) - 1))] = base + id;
+      const int one = __shfl_sync(kFull, base + id, set ? __ffs(set) - 1 : 0);
+      const int padded = (total + kAhead - 1) / kAhead * kAhead;
+      if (lane >= total && lane < padded) keys[i][lane] = one;
+      if (lane == 0) count[i] = total;
+    }
+    __syncthreads();
+  }
+};
+
+// A group of L lanes per (row, head).  What every kernel over query rows
+// starts from.
 template <typename T, int L>
-__global__ void __launch_bounds__(kBlock)
-    neighbor_forward_kernel(const __grid_constant__ NeighborArgs a) {
-  constexpr int V = Vec<T>::V;
-  const long long unit =
-      ((long long)blockIdx.x * kBlock + threadIdx.x) / L;
-  const int j = threadIdx.x % L;
-  const long long total = a.n_q * a.heads;
-  const bool live = unit < total;
-  const long long row = live ? unit / a.heads : 0;
-  const int h = live ? (int)(unit - row * a.heads) : 0;
-  const bool mine = live && j * V < a.dim;
-  float q[V], acc[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) q[i] = acc[i] = 0.f;
-  if (mine)
-    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
-                       static_cast<const T*>(a.q) + row * a.q_row +
-                       h * a.q_head + j * V), q);
-  const int scene = scene_of(a.q_seg, a.scenes, (int)row);
-  const int base = __ldg(a.k_seg + scene);
-  const int n = live ? __ldg(a.k_seg + scene + 1) - base : 0;
-  const int hk = h / a.group;
-  const T* k = static_cast<const T*>(a.k) + hk * a.k_head + j * V;
-  const T* v = static_cast<const T*>(a.v) + hk * a.v_head + j * V;
-  const int* ids = a.ids + row * a.width;
-  const int first = __ldg(ids);
-  float m = -kInf, l = 0.f;
-  bool any = false;
-  for (int j0 = 0; j0 < a.width; j0 += kAhead) {
+struct Group {
+  static constexpr int V = Vec<T>::V;
+  long long unit, row;
+  int h, j, n;        // head; lane of the group; entries
+  const int* keys;
+  bool live, mine;    // a unit of its own; a vector of its own
+  const T *k, *v;
+
+  __device__ __forceinline__ Group(
+      const NeighborArgs& a, RowLists<kBlock / L + 1>& lists) {
+    const long long unit0 = (long long)blockIdx.x * (kBlock / L);
+    const long long total = a.n_q * a.heads;
+    const long long last = min(unit0 + kBlock / L, total) - 1;
+    const long long row0 = unit0 / a.heads;
+    lists.fill(a, row0, (int)(last / a.heads - row0) + 1);
+    unit = unit0 + threadIdx.x / L;
+    j = threadIdx.x % L;
+    live = unit < total;
+    row = live ? unit / a.heads : row0;
+    h = live ? (int)(unit - row * a.heads) : 0;
+    mine = live && j * V < a.dim;
+    keys = lists.keys[row - row0];
+    n = live ? lists.count[row - row0] : 0;
+    const int hk = h / a.group;
+    k = static_cast<const T*>(a.k) + hk * a.k_head + j * V;
+    v = static_cast<const T*>(a.v) + hk * a.v_head + j * V;
+  }
+
+  // The vectors of kAhead entries from j0 on.
+  __device__ __forceinline__ void load(const NeighborArgs& a, int j0,
+                                       uint4* ku, uint4* vu) const {
     int at[kAhead];
-    entries(a, ids, j0, first, base, n, at);
-    bool here = false;
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) here |= at[t] >= 0;
-    if (!__any_sync(kFull, here)) continue;
-    any |= here;
-    uint4 ku[kAhead], vu[kAhead];
+    for (int t = 0; t < kAhead; t += 4)
+      *reinterpret_cast<int4*>(at + t) =
+          *reinterpret_cast<const int4*>(keys + j0 + t);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
       ku[t] = vu[t] = make_uint4(0, 0, 0, 0);
-      if (mine && at[t] >= 0) {
+      if (mine && j0 < n) {
         ku[t] = __ldg(reinterpret_cast<const uint4*>(k + at[t] * a.k_row));
         vu[t] = __ldg(reinterpret_cast<const uint4*>(v + at[t] * a.v_row));
       }
     }
+  }
+};
+
+template <typename T, int L>
+__global__ void __launch_bounds__(kBlock)
+    neighbor_forward_kernel(const __grid_constant__ NeighborArgs a) {
+  __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
+  const Group<T, L> g(a, lists);
+  Pairs<T> q, acc;
+  q.clear();
+  acc.clear();
+  if (g.mine)
+    q = Pairs<T>(vector_at<T>(a.q, g.row * a.q_row + g.h * a.q_head +
+                                       g.j * Vec<T>::V));
+  float m = -kInf, l = 0.f;
+  for (int j0 = 0; __any_sync(kFull, j0 < g.n); j0 += kAhead) {
+    uint4 ku[kAhead], vu[kAhead];
+    g.load(a, j0, ku, vu);
     float s[kAhead], top = m;
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      s[t] = group_sum<L>(dot<T, V>(ku[t], q)) * a.scale_log2e;
-      if (at[t] < 0) s[t] = -kInf;
+      s[t] = group_sum<L>(Pairs<T>(ku[t]).dot(q)) * a.scale_log2e;
+      if (j0 + t >= g.n) s[t] = -kInf;
       top = fmaxf(top, s[t]);
     }
     const float shift = top == -kInf ? 0.f : top;
     const float keep = exp2_fast(m - shift);
     m = top;
     l *= keep;
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] *= keep;
+    acc.scale(keep);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      if (at[t] < 0) continue;  // a masked score of NaN counts for nothing
       const float p = exp2_fast(s[t] - shift);
       l += p;
-      float f[V];
-      Vec<T>::unpack(vu[t], f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(p, f[i], acc[i]);
+      // behind the last entry: nothing, whatever the first one's value holds
+      if (j0 + t < g.n) acc.add(p, Pairs<T>(vu[t]));
     }
   }
-  if (!live) return;
-  if (mine) {
-    const float r = any ? 1.f / l : 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = any ? acc[i] * r : 0.f;
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * a.o_row +
-                              h * a.o_head + j * V) = Vec<T>::pack(acc);
+  if (!g.live) return;
+  if (g.mine) {
+    if (g.n) acc.scale(1.f / l); else acc.clear();
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + g.row * a.o_row +
+                              g.h * a.o_head + g.j * Vec<T>::V) = acc.pack();
   }
-  if (j == 0 && a.lse_out)
-    a.lse_out[unit] = any ? (m + log2f(l)) * kLn2 : -kInf;
+  if (g.j == 0 && a.lse_out)
+    a.lse_out[g.unit] = g.n ? (m + log2f(l)) * kLn2 : -kInf;
 }
 
 // dq, and delta for the keys' pass.
 template <typename T, int L>
 __global__ void __launch_bounds__(kBlock)
     neighbor_dq_kernel(const __grid_constant__ NeighborArgs a) {
-  constexpr int V = Vec<T>::V;
-  const long long unit =
-      ((long long)blockIdx.x * kBlock + threadIdx.x) / L;
-  const int j = threadIdx.x % L;
-  const long long total = a.n_q * a.heads;
-  const bool live = unit < total;
-  const long long row = live ? unit / a.heads : 0;
-  const int h = live ? (int)(unit - row * a.heads) : 0;
-  const bool mine = live && j * V < a.dim;
-  float q[V], d[V], acc[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) q[i] = d[i] = acc[i] = 0.f;
+  __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
+  const Group<T, L> g(a, lists);
+  const int at = g.j * Vec<T>::V;
+  Pairs<T> q, d, acc;
+  q.clear();
+  d.clear();
+  acc.clear();
   float part = 0.f;
-  if (mine) {
-    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
-                       static_cast<const T*>(a.q) + row * a.q_row +
-                       h * a.q_head + j * V), q);
-    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
-                       static_cast<const T*>(a.dout) + row * a.d_row +
-                       h * a.d_head + j * V), d);
-    part = dot<T, V>(*reinterpret_cast<const uint4*>(
-                         static_cast<const T*>(a.out) + row * a.o_row +
-                         h * a.o_head + j * V), d);
+  if (g.mine) {
+    q = Pairs<T>(vector_at<T>(a.q, g.row * a.q_row + g.h * a.q_head + at));
+    d = Pairs<T>(vector_at<T>(a.dout, g.row * a.d_row + g.h * a.d_head + at));
+    part = Pairs<T>(vector_at<T>(a.out, g.row * a.o_row + g.h * a.o_head + at))
+               .dot(d);
   }
   const float delta = group_sum<L>(part);
-  if (live && j == 0) a.delta[unit] = delta;
-  const float lse2 = live ? __ldg(a.lse + unit) * kLog2e : 0.f;
-  const int scene = scene_of(a.q_seg, a.scenes, (int)row);
-  const int base = __ldg(a.k_seg + scene);
-  const int n = live ? __ldg(a.k_seg + scene + 1) - base : 0;
-  const int hk = h / a.group;
-  const T* k = static_cast<const T*>(a.k) + hk * a.k_head + j * V;
-  const T* v = static_cast<const T*>(a.v) + hk * a.v_head + j * V;
-  const int* ids = a.ids + row * a.width;
-  const int first = __ldg(ids);
-  for (int j0 = 0; j0 < a.width; j0 += kAhead) {
-    int at[kAhead];
-    entries(a, ids, j0, first, base, n, at);
-    bool here = false;
-#pragma unroll
-    for (int t = 0; t < kAhead; ++t) here |= at[t] >= 0;
-    if (!__any_sync(kFull, here)) continue;
+  if (g.live && g.j == 0) a.delta[g.unit] = delta;
+  const float lse2 = g.live ? __ldg(a.lse + g.unit) * kLog2e : 0.f;
+  for (int j0 = 0; __any_sync(kFull, j0 < g.n); j0 += kAhead) {
     uint4 ku[kAhead], vu[kAhead];
+    g.load(a, j0, ku, vu);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      ku[t] = vu[t] = make_uint4(0, 0, 0, 0);
-      if (mine && at[t] >= 0) {
-        ku[t] = __ldg(reinterpret_cast<const uint4*>(k + at[t] * a.k_row));
-        vu[t] = __ldg(reinterpret_cast<const uint4*>(v + at[t] * a.v_row));
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < kAhead; ++t) {
-      float f[V];
-      Vec<T>::unpack(ku[t], f);
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) s = fmaf(f[i], q[i], s);
-      s = group_sum<L>(s);
-      const float dp = group_sum<L>(dot<T, V>(vu[t], d));
-      if (at[t] < 0) continue;
+      const Pairs<T> k(ku[t]);
+      const float s = group_sum<L>(k.dot(q));
+      const float dp = group_sum<L>(Pairs<T>(vu[t]).dot(d));
       const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2));
-      const float ds = p * (dp - delta);
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(ds, f[i], acc[i]);
+      if (j0 + t < g.n) acc.add(p * (dp - delta), k);
     }
   }
-  if (mine) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] *= a.scale;
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.dq) +
-                              unit * a.dim + j * V) = Vec<T>::pack(acc);
+  if (g.mine) {
+    acc.scale(a.scale);
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.dq) + g.unit * a.dim + at) =
+        acc.pack();
   }
 }
 
 // dk and dv: a warp per (key, head of keys); its 32 / L groups take the key's
 // (entry, query head) pairs in turn and are added up at the end.
 template <typename T, int L>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, 8)
     neighbor_dkv_kernel(const __grid_constant__ NeighborArgs a) {
   constexpr int V = Vec<T>::V;
   constexpr int G = 32 / L;
-  constexpr int kDeep = 4;
+  // Entries of a group in flight: more warps (64 registers) are worth more
+  // here (4 with 96 registers: 571 us of the training case, so: 503).
+  constexpr int kDeep = 2;
   const long long unit =
       ((long long)blockIdx.x * kBlock + threadIdx.x) >> 5;
   if (unit >= a.n_k * a.kv_heads) return;  // the whole warp
@@ -252,80 +290,67 @@ __global__ void __launch_bounds__(kBlock)
   const long long key = unit / a.kv_heads;
   const int hk = (int)(unit - key * a.kv_heads);
   const bool mine = j * V < a.dim;
-  float k[V], v[V], dk[V], dv[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) k[i] = v[i] = dk[i] = dv[i] = 0.f;
+  Pairs<T> k, v, dk, dv;
+  k.clear();
+  v.clear();
+  dk.clear();
+  dv.clear();
   if (mine) {
-    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
-                       static_cast<const T*>(a.k) + key * a.k_row +
-                       hk * a.k_head + j * V), k);
-    Vec<T>::unpack(*reinterpret_cast<const uint4*>(
-                       static_cast<const T*>(a.v) + key * a.v_row +
-                       hk * a.v_head + j * V), v);
+    k = Pairs<T>(vector_at<T>(a.k, key * a.k_row + hk * a.k_head + j * V));
+    v = Pairs<T>(vector_at<T>(a.v, key * a.v_row + hk * a.v_head + j * V));
   }
-  const int from = __ldg(a.starts + key);
-  const long long pairs =
-      (long long)(__ldg(a.starts + key + 1) - from) * a.group;
-  for (long long t0 = 0; t0 < pairs; t0 += G * kDeep) {
-    uint4 qu[kDeep], du[kDeep];
-    float lse2[kDeep], delta[kDeep];
+  const int from = __ldg(a.starts + key), to = __ldg(a.starts + key + 1);
+  for (int e0 = from; e0 < to; e0 += 32) {
+    // an entry's row and its values in a lane each
+    const int n = min(32, to - e0);
+    const int mine_row = lane < n ? __ldg(a.order + e0 + lane) : 0;
+    for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
+      float mine_lse = 0.f, mine_delta = 0.f;
+      if (lane < n) {
+        const long long at = (long long)mine_row * a.heads + h;
+        mine_lse = __ldg(a.lse + at) * kLog2e;
+        mine_delta = __ldg(a.delta + at);
+      }
+      for (int t0 = 0; t0 < n; t0 += G * kDeep) {
+        uint4 qu[kDeep], du[kDeep];
+        float lse2[kDeep], delta[kDeep];
 #pragma unroll
-    for (int t = 0; t < kDeep; ++t) {
-      const long long at = t0 + t * G + who;
-      qu[t] = du[t] = make_uint4(0, 0, 0, 0);
-      lse2[t] = kInf;  // absent: p = 0
-      delta[t] = 0.f;
-      if (at < pairs) {
-        const long long e = at / a.group;
-        const int h = hk * a.group + (int)(at - e * a.group);
-        const long long row = __ldg(a.order + from + e);
-        lse2[t] = __ldg(a.lse + row * a.heads + h) * kLog2e;
-        delta[t] = __ldg(a.delta + row * a.heads + h);
-        if (mine) {
-          qu[t] = __ldg(reinterpret_cast<const uint4*>(
-              static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head +
-              j * V));
-          du[t] = __ldg(reinterpret_cast<const uint4*>(
-              static_cast<const T*>(a.dout) + row * a.d_row + h * a.d_head +
-              j * V));
+        for (int t = 0; t < kDeep; ++t) {
+          const int e = t0 + t * G + who;
+          const long long row = __shfl_sync(kFull, mine_row, e & 31);
+          lse2[t] = __shfl_sync(kFull, mine_lse, e & 31);
+          delta[t] = __shfl_sync(kFull, mine_delta, e & 31);
+          qu[t] = du[t] = make_uint4(0, 0, 0, 0);
+          if (mine && e < n) {
+            qu[t] = vector_at<T>(a.q, row * a.q_row + h * a.q_head + j * V);
+            du[t] = vector_at<T>(a.dout, row * a.d_row + h * a.d_head + j * V);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kDeep; ++t) {
+          const Pairs<T> q(qu[t]), d(du[t]);
+          const float s = group_sum<L>(q.dot(k)), dp = group_sum<L>(d.dot(v));
+          if (t0 + t * G + who >= n) continue;
+          const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2[t]));
+          dk.add(p * (dp - delta[t]), q);
+          dv.add(p, d);
         }
       }
     }
-#pragma unroll
-    for (int t = 0; t < kDeep; ++t) {
-      float f[V], g[V], s = 0.f, dp = 0.f;
-      Vec<T>::unpack(qu[t], f);
-      Vec<T>::unpack(du[t], g);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        s = fmaf(f[i], k[i], s);
-        dp = fmaf(g[i], v[i], dp);
-      }
-      s = group_sum<L>(s);
-      dp = group_sum<L>(dp);
-      if (t0 + t * G + who >= pairs) continue;
-      const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2[t]));
-      const float ds = p * (dp - delta[t]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        dk[i] = fmaf(ds, f[i], dk[i]);
-        dv[i] = fmaf(p, g[i], dv[i]);
-      }
-    }
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < Pairs<T>::N; ++i) {
 #pragma unroll
     for (int o = L; o < 32; o <<= 1) {
-      dk[i] += __shfl_xor_sync(kFull, dk[i], o);
-      dv[i] += __shfl_xor_sync(kFull, dv[i], o);
+      dk.v[i] = tc::add2(dk.v[i], __shfl_xor_sync(kFull, dk.v[i], o));
+      dv.v[i] = tc::add2(dv.v[i], __shfl_xor_sync(kFull, dv.v[i], o));
     }
-    dk[i] *= a.scale;
   }
   if (who == 0 && mine) {
+    dk.scale(a.scale);
     const long long at = unit * a.dim + j * V;
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.dk) + at) = Vec<T>::pack(dk);
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.dv) + at) = Vec<T>::pack(dv);
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.dk) + at) = dk.pack();
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.dv) + at) = dv.pack();
   }
 }
 
