@@ -42,24 +42,25 @@ def check(code, what):
 def rows_of(t, what, shape, dtype, device):
     """``(data, row stride, head stride)`` of a CUDA tensor of rows of heads;
     anything but the expected shape, type and device raises."""
-    if not (
-        isinstance(t, torch.Tensor)
-        and t.is_cuda
-        and t.get_device() == device
-        and t.dtype == dtype
-        and t.shape == shape
-        and (t.stride(2) == 1 or t.numel() == 0)
-    ):
+    try:
+        row, head, element = t.stride()
+        fits = t.shape == shape and t.dtype is dtype and t.get_device() == device and (element == 1 or not t.numel())
+    except (AttributeError, ValueError):
+        fits = False
+    if not fits:
         raise ValueError(
             f"{what} must be a {dtype} tensor of shape {tuple(shape)} on the current CUDA device, its last dimension contiguous"
         )
-    return t.data_ptr(), t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
+    return t.data_ptr(), row if shape[0] > 1 else 0, head if shape[1] > 1 else 0
+
+
+_STEP = {torch.float32: 3, torch.float16: 7, torch.bfloat16: 7}  # 16 bytes less one element
 
 
 def vector_rows_of(t, what, shape, dtype, device):
     """``rows_of`` for kernels that take 16 bytes at a time."""
     data, row, head = found = rows_of(t, what, shape, dtype, device)
-    if (data | row * t.element_size() | head * t.element_size()) & 15:
+    if data & 15 or (row | head) & _STEP[dtype]:
         raise ValueError(f"{what} must start on 16 bytes and have row and head strides that are multiples of 16 bytes")
     return found
 

@@ -66,32 +66,37 @@ class ScenePairs:
 class _Call:
     """The checked arguments that one attention call and its gradient share."""
 
+    __slots__ = ("what", "device", "stream", "pairs", "dtype", "q_shape", "k_shape", "on", "sizes", "rows", "mask", "ids",
+                 "width", "padded")
+
     def __init__(self, what, q, k, v, pairs, scale, types):
-        if not (isinstance(q, torch.Tensor) and q.ndim == 3 and isinstance(k, torch.Tensor) and k.ndim == 3
-                and q.is_cuda and q.dtype in types):
+        try:
+            (n_q, heads, dim), (n_k, kv_heads, _) = q.shape, k.shape
+            fits = q.is_cuda and q.dtype in types
+        except (AttributeError, ValueError):
+            fits = False
+        if not fits:
             raise ValueError(f"{what} needs CUDA (N, heads, dim) rows of one type among {[str(t) for t in types]}")
-        self.device, self.stream = current_stream()
-        if not isinstance(pairs, ScenePairs) or pairs.device != self.device:
+        self.device, self.stream = device, _ = current_stream()
+        if not isinstance(pairs, ScenePairs) or pairs.device != device:
             raise ValueError(f"{what} needs ScenePairs made on the current device")
-        n_q, self.heads, self.dim = q.shape
-        n_k, self.kv_heads = k.shape[:2]
-        if not (8 <= self.dim <= MAX_DIM and self.dim % 8 == 0):
+        if not 8 <= dim <= MAX_DIM or dim & 7:
             raise ValueError("the head size must be a multiple of 8, at most 128")
-        if not (self.kv_heads and self.heads and self.heads % self.kv_heads == 0):
+        if not (kv_heads and heads and heads % kv_heads == 0):
             raise ValueError("the query heads must be a multiple of the keys' heads")
-        if types is _HALF and self.heads // self.kv_heads > MAX_GROUP:
+        if types is _HALF and heads // kv_heads > MAX_GROUP:
             raise ValueError("at most 64 query heads share a head of keys")
-        if (n_q, n_k) != (pairs.n_q, pairs.n_k):
+        if n_q != pairs.n_q or n_k != pairs.n_k:
             raise ValueError("query and key rows must be those of the pairs' offsets")
         if scale is None:
-            scale = self.dim ** -0.5
+            scale = dim ** -0.5
         if not 2.0**-24 <= scale <= 2.0**24:
             raise ValueError("scale must be positive, from 2^-24 to 2^24")
-        self.what, self.dtype, self.pairs, self.scale = what, q.dtype, pairs, scale
-        self.q_shape, self.k_shape = q.shape, torch.Size((n_k, self.kv_heads, self.dim))
-        self.rows = [self.rows_of(t, n, s) for t, n, s in (
-            (q, "q", self.q_shape), (k, "k", self.k_shape), (v, "v", self.k_shape))]
-        self.q_device = q.device
+        self.what, self.dtype, self.pairs, self.on = what, q.dtype, pairs, q.device
+        self.q_shape, self.k_shape = (n_q, heads, dim), (n_k, kv_heads, dim)
+        self.sizes = (ft.TYPES[q.dtype], pairs.scenes, n_q, n_k, pairs.max_q, pairs.max_k, heads, kv_heads, dim, scale)
+        self.rows = self.rows_of(q, "q", self.q_shape) + self.rows_of(k, "k", self.k_shape) + self.rows_of(
+            v, "v", self.k_shape)
         self.mask = self.ids = self.width = self.padded = 0
 
     def rows_of(self, t, name, shape):
@@ -100,65 +105,70 @@ class _Call:
     def set_mask(self, mask):
         if mask is None:
             return
-        if not (isinstance(mask, torch.Tensor) and mask.is_cuda and mask.get_device() == self.device
+        if not (isinstance(mask, torch.Tensor) and mask.get_device() == self.device
                 and mask.dtype in (torch.bool, torch.uint8) and mask.shape == (self.pairs.n_k,)
                 and mask.is_contiguous()):
             raise ValueError("mask must be contiguous CUDA bool (N_k,): the keys that may be read")
         self.mask = mask.data_ptr()
 
     def set_ids(self, ids, padded):
-        if not (isinstance(ids, torch.Tensor) and ids.is_cuda and ids.get_device() == self.device
-                and ids.dtype == torch.int32 and ids.ndim == 2 and ids.shape[0] == self.pairs.n_q
+        if not (isinstance(ids, torch.Tensor) and ids.get_device() == self.device
+                and ids.dtype is torch.int32 and ids.ndim == 2 and ids.shape[0] == self.pairs.n_q
                 and 1 <= ids.shape[1] <= MAX_WIDTH and ids.is_contiguous()):
             raise ValueError("rows must be contiguous CUDA int32 (N_q, K) with K in [1,32]")
-        self.ids, self.width, self.padded = ids.data_ptr(), ids.shape[1], int(bool(padded))
+        self.ids, self.width, self.padded = ids.data_ptr(), ids.shape[1], 1 if padded else 0
 
     def lse_of(self, lse):
-        if not (isinstance(lse, torch.Tensor) and lse.is_cuda and lse.get_device() == self.device
-                and lse.dtype == torch.float32 and lse.shape == self.q_shape[:2] and lse.is_contiguous()):
+        if not (isinstance(lse, torch.Tensor) and lse.get_device() == self.device
+                and lse.dtype is torch.float32 and lse.shape == self.q_shape[:2] and lse.is_contiguous()):
             raise ValueError("lse must be contiguous CUDA FP32 (N_q, heads)")
         return lse.data_ptr()
-
-    def empty(self, shape, dtype=None):
-        return torch.empty(shape, dtype=dtype or self.dtype, device=self.q_device)
 
     def run(self, entry, workspace, out, dout, lse, grads):
         p = self.pairs
 
         def pack(at, size):
-            return ft.pack_attention(
-                ft.TYPES[self.dtype], p.scenes, p.n_q, p.n_k, p.max_q, p.max_k, self.heads, self.kv_heads, self.dim,
-                self.scale, *self.rows[0], *self.rows[1], *self.rows[2], *out, *dout, lse, *grads, p._q_at, p._k_at,
-                self.mask, self.ids, self.width, self.padded, at, size, p._error_at, self.stream,
-            )
+            return ft.pack_attention(*self.sizes, *self.rows, *out, *dout, lse, *grads, p._q_at, p._k_at, self.mask, self.ids,
+                                     self.width, self.padded, at, size, p._error_at, self.stream)
 
-        args, buffer = pack(0, 0), None
+        args = pack(0, 0)
         if workspace is not None:
             size = workspace(args)
-            ft.check(min(size, 0), self.what)
+            if size < 0:
+                ft.check(size, self.what)
             if size:
                 # private to this call: calls on several streams, and
                 # captured ones, never share a workspace
-                buffer = self.empty((size,), torch.uint8)
+                buffer = torch.empty(size, dtype=torch.uint8, device=self.on)
                 args = pack(buffer.data_ptr(), size)
-        ft.check(entry(args), self.what)
+        code = entry(args)
+        if code:
+            ft.check(code, self.what)
 
-    def forward(self, entry, workspace, out, return_lse, taken):
+    def forward(self, entry, workspace, out, return_lse, inputs):
         if out is None:
-            out = self.empty(self.q_shape)
-        place = self.rows_of(out, "out", self.q_shape)
-        ft.check_written(out, "out")
-        if out.numel() and out.data_ptr() in taken:
-            raise ValueError("out must not overlap the inputs")
-        lse = self.empty(self.q_shape[:2], torch.float32) if return_lse else None
-        self.run(entry, workspace, place, (0, 0, 0), lse.data_ptr() if return_lse else 0, (0, 0, 0))
-        return (out, lse) if return_lse else out
+            out = torch.empty(self.q_shape, dtype=self.dtype, device=self.on)
+            _, heads, dim = self.q_shape
+            place = (out.data_ptr(), heads * dim, dim)
+        else:
+            place = self.rows_of(out, "out", self.q_shape)
+            ft.check_written(out, "out")
+            if place[0] and place[0] in [t.data_ptr() for t in inputs]:
+                raise ValueError("out must not overlap the inputs")
+        if not return_lse:
+            self.run(entry, workspace, place, (0, 0, 0), 0, (0, 0, 0))
+            return out
+        lse = torch.empty(self.q_shape[:2], dtype=torch.float32, device=self.on)
+        self.run(entry, workspace, place, (0, 0, 0), lse.data_ptr(), (0, 0, 0))
+        return out, lse
 
     def backward(self, entry, workspace, dout, out, lse):
-        grads = self.empty(self.q_shape), self.empty(self.k_shape), self.empty(self.k_shape)
+        dq = torch.empty(self.q_shape, dtype=self.dtype, device=self.on)
+        dk = torch.empty(self.k_shape, dtype=self.dtype, device=self.on)
+        dv = torch.empty(self.k_shape, dtype=self.dtype, device=self.on)
         self.run(entry, workspace, self.rows_of(out, "out", self.q_shape), self.rows_of(dout, "dout", self.q_shape),
-                 self.lse_of(lse), [g.data_ptr() for g in grads])
-        return grads
+                 self.lse_of(lse), (dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
+        return dq, dk, dv
 
 
 _HALF = (torch.bfloat16, torch.float16)
@@ -166,15 +176,13 @@ _ALL = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _wants_grad(out, *tensors):
-    return out is None and torch.is_grad_enabled() and any(
-        isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+    return out is None and any(getattr(t, "requires_grad", False) for t in tensors) and torch.is_grad_enabled()
 
 
 def _cross(q, k, v, pairs, mask, scale, out, return_lse):
     call = _Call("cross attention", q, k, v, pairs, scale, _HALF)
     call.set_mask(mask)
-    return call.forward(ft.lib.cross_attention, ft.lib.cross_attention_workspace, out, return_lse,
-                        (q.data_ptr(), k.data_ptr(), v.data_ptr()))
+    return call.forward(ft.lib.cross_attention, ft.lib.cross_attention_workspace, out, return_lse, (q, k, v))
 
 
 def cross_attention(q, k, v, pairs, mask=None, scale=None, out=None, return_lse=False):
@@ -208,7 +216,7 @@ def cross_attention_grad(dout, q, k, v, out, lse, pairs, mask=None, scale=None):
 def _neighbor(q, k, v, rows, pairs, padded, scale, out, return_lse):
     call = _Call("neighbor attention", q, k, v, pairs, scale, _ALL)
     call.set_ids(rows, padded)
-    return call.forward(ft.lib.neighbor_attention, None, out, return_lse, (q.data_ptr(), k.data_ptr(), v.data_ptr()))
+    return call.forward(ft.lib.neighbor_attention, None, out, return_lse, (q, k, v))
 
 
 def neighbor_attention(q, k, v, rows, pairs, padded=True, scale=None, out=None, return_lse=False):

@@ -74,35 +74,45 @@ class Rotary:
             raise ValueError("amplitude must be finite")
         self.part, self.axes, self.layout, self.amplitude = part, axes, layout, amplitude
         self.pairs = part // (2 * axes)
+        self._interleaved = layout == "interleaved"
         f = frequencies(self.pairs, base, scaling, factor, length)
         self._turns = (ctypes.c_double * self.pairs)(*[v / (2 * math.pi) / unit for v in f])
         self._turns_at = ctypes.addressof(self._turns)
 
     def _run(self, x, positions, out, transposed):
-        if not (isinstance(x, torch.Tensor) and x.is_cuda and x.ndim == 3 and x.dtype in ft.TYPES and x.shape[1] > 0
-                and self.part <= x.shape[2] <= MAX_DIM):
+        try:
+            rows, heads, dim = shape = x.shape
+            fits = x.is_cuda and x.dtype in ft.TYPES and heads > 0 and self.part <= dim <= MAX_DIM
+        except (AttributeError, ValueError):
+            fits = False
+        if not fits:
             raise ValueError("rows must be CUDA FP32, FP16 or BF16 (N, heads, dim) with dim from part to 4096")
         device, stream = current_stream()
-        rows, heads, dim = x.shape
-        place = ft.rows_of(x, "rows", x.shape, x.dtype, device)
-        if not (
-            isinstance(positions, torch.Tensor)
-            and positions.is_cuda
-            and positions.get_device() == device
-            and positions.dtype in ft.POSITION_TYPES
-            and (positions.shape == (rows, self.axes) or (self.axes == 1 and positions.shape == (rows,)))
-        ):
+        dtype = x.dtype
+        place = ft.rows_of(x, "rows", shape, dtype, device)
+        try:
+            kind = ft.POSITION_TYPES.get(positions.dtype, -1)
+            n, *axes = positions.shape
+            fits = kind >= 0 and positions.get_device() == device and n == rows and (
+                axes == [self.axes] or (self.axes == 1 and not axes))
+        except (AttributeError, ValueError):
+            fits = False
+        if not fits:
             raise ValueError("positions must be CUDA FP32, int32 or int64 (N, axes) on the rows' device")
         if out is None:
-            out = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device)
-        to = ft.rows_of(out, "out", x.shape, x.dtype, device)
-        ft.check_written(out, "out")
+            out = torch.empty(shape, dtype=dtype, device=x.device)
+            to = (out.data_ptr(), heads * dim, dim)
+        else:
+            to = ft.rows_of(out, "out", shape, dtype, device)
+            ft.check_written(out, "out")
+        steps = positions.stride()
         args = ft.pack_rotary(
-            ft.TYPES[x.dtype], rows, heads, dim, *place, *to, positions.data_ptr(), ft.POSITION_TYPES[positions.dtype],
-            positions.stride(0), positions.stride(1) if positions.ndim == 2 else 0, self.axes, self.pairs,
-            self._turns_at, self.amplitude, self.layout == "interleaved", transposed, stream,
+            ft.TYPES[dtype], rows, heads, dim, *place, *to, positions.data_ptr(), kind, steps[0], steps[1] if axes else 0,
+            self.axes, self.pairs, self._turns_at, self.amplitude, self._interleaved, transposed, stream,
         )
-        ft.check(ft.lib.rotary_positions(args), "rotary positions")
+        code = ft.lib.rotary_positions(args)
+        if code:
+            ft.check(code, "rotary positions")
         return out
 
     def __call__(self, x, positions, out=None):
@@ -110,7 +120,7 @@ class Rotary:
         head strides) turned by ``positions`` (FP32, int32 or int64
         (N, axes), or (N,) for one axis).  ``out`` may be ``x`` itself, else it does not
         overlap it.  Differentiable in ``x`` when ``out`` is not given."""
-        if out is None and isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        if out is None and getattr(x, "requires_grad", False) and torch.is_grad_enabled():
             return _Turn.apply(x, positions, self)
         return self._run(x, positions, out, False)
 
