@@ -77,12 +77,12 @@ struct BackMaps {
 enum Bar {
   kTileFull = 0,  // [stage] a walked tile is there
   kTileFree = 4,  // [stage] its products are complete
-  kTileRaw = 8,   // a tile loaded, rows to be cleared
-  kScores = 9,    // S and dP are complete
-  kRead = 10,     // they are in registers (a count per warp)
-  kWeights = 11,  // P and dS are there (a count per warp)
-  kOutput = 12,   // the second products are complete
-  kBars = 13
+  kTileRaw = 8,   // [stage] a tile loaded, rows to be cleared
+  kScores = 12,   // S and dP are complete
+  kRead = 13,     // they are in registers (a count per warp)
+  kWeights = 14,  // P and dS are there (a count per warp)
+  kOutput = 15,   // the second products are complete
+  kBars = 16
 };
 
 // Factors that P and dS carry (2^x).
@@ -180,9 +180,93 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
   // lse is below 2^16; of delta
   const int s_exp = a.scale_exponent, d_exp = 8;
 
+  // The loading warp: a tile's copies, and what is left to do when they are
+  // there.
+  const int panels = a.dim > 64 ? 2 : 1;
+  int cleared = 0;  // a bit per stage: the phase of its raw barrier
+  uint4 values[W / 32];
+  const uint4 nothing =  // lse = inf: P = 0
+      make_uint4(pack2<T>(-kInf, 0.f), 0, 0, 0);
+  auto load_values = [&](int t) {
+    const int first = (begin + t) * each;
+    const long long at = ((long long)hk * a.n_q + q0) * a.group;
+#pragma unroll
+    for (int i = 0; i < W / 32; ++i) {
+      const int r = first + i * 32 + lane;
+      const bool there = t < nt && i * 32 + lane < each && r < n;
+      values[i] = there ? a.row_values[at + r] : nothing;
+    }
+  };
+  auto whole = [&](int t, uint32_t* open) {
+    const int at = (begin + t) * each;
+    if constexpr (kKeysPass) {
+      key_words<W>(open, nullptr, 0, min(n - at, each));
+      return n - at >= each;
+    } else {
+      key_words<W>(open, mask, at, nk);
+      bool all = true;
+#pragma unroll
+      for (int i = 0; i < W / 32; ++i) all &= open[i] == 0xffffffffu;
+      return all;
+    }
+  };
+  auto issue = [&](int t) {
+    const int stage = t % S::kStages;
+    const int at = (begin + t) * each;
+    const uint32_t t1 = y1 + stage * S::kTile, t2 = y2 + stage * S::kTile;
+    uint32_t open[W / 32];
+    const int full = (whole(t, open) ? kTileFull : kTileRaw) + stage;
+    if (t >= S::kStages) wait(kTileFree + stage, t / S::kStages - 1);
+    __syncwarp();
+    if (tc::elect()) {
+      tc::barrier_expect(bar(full), 2 * panels * each * 128);
+      const int head = kKeysPass ? hk * a.group : hk;
+      const int row = kKeysPass ? q0 + at / a.group : k0 + at;
+      for (int p = 0; p < panels; ++p) {
+        tc::copy_box(t1 + p * W * 128, &maps.y1, bar(full), p * 64, head, row);
+        tc::copy_box(t2 + p * W * 128, &maps.y2, bar(full), p * 64, head, row);
+      }
+    }
+    __syncwarp();
+  };
+  auto finish = [&](int t) {
+    const int stage = t % S::kStages;
+    if constexpr (kKeysPass) {
+#pragma unroll
+      for (int i = 0; i < W / 32; ++i) {
+        const uint32_t to =
+            stage * S::kTileMore + tc::narrow_offset(i * 32 + lane, 0);
+        store(y1_more + to, values[i].x, values[i].y);
+        store(y2_more + to, values[i].z, values[i].w);
+      }
+      // the next tile's are on their way while its place is waited for
+      load_values(t + 1);
+    }
+    uint32_t open[W / 32];
+    const bool all = whole(t, open);
+    if (!all) {
+      wait(kTileRaw + stage, cleared >> stage);
+      cleared ^= 1 << stage;
+      __syncwarp();
+      clear_rows<W>(y1 + stage * S::kTile, panels, open);
+      if constexpr (kKeysPass)
+        clear_rows<W>(y2 + stage * S::kTile, panels, open);
+    }
+    if (!all || kKeysPass) {
+      tc::fence_shared();
+      __syncwarp();
+      // in the keys' pass a tile is there with its copies and its values
+      if (lane == 0) {
+        tc::barrier_arrive(bar(kTileFull + stage));
+        if (!all && kKeysPass) tc::barrier_arrive(bar(kTileFull + stage));
+      }
+    }
+  };
+
   if (nt > 0) {
     if (warp == kRowWarps) {
       tc::tmem_alloc(tc::smem_address(&tmem_at), S::kColumns);
+    } else if (warp == kRowWarps + 1) {
       if (lane == 0) {
         for (int i = 0; i < kBars; ++i)
           tc::barrier_init(bar(i), i == kRead || i == kWeights ? kRowWarps
@@ -191,6 +275,9 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         tc::barriers_ready();
       }
       __syncwarp();
+      // the first tiles come while the block gets ready
+      for (int t = 0; t < S::kStages && t < nt; ++t) issue(t);
+      if constexpr (kKeysPass) load_values(0);
     } else if (warp < kRowWarps) {
       const Chunks c = chunks_of(a.dim, tid, kRowWarps * 32);
       if constexpr (kKeysPass) {
@@ -267,78 +354,9 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
   }
 
   if (warp == kRowWarps + 1) {
-    const int panels = a.dim > 64 ? 2 : 1;
-    int cleared = 0;
-    // the values of the next tile's rows are on their way while this one's
-    // place is waited for
-    uint4 values[W / 32];
-    const uint4 nothing =  // lse = inf: P = 0
-        make_uint4(pack2<T>(-kInf, 0.f), 0, 0, 0);
-    auto load_values = [&](int t) {
-      const int first = (begin + t) * each;
-      const long long at = ((long long)hk * a.n_q + q0) * a.group;
-#pragma unroll
-      for (int i = 0; i < W / 32; ++i) {
-        const int r = first + i * 32 + lane;
-        const bool there = t < nt && i * 32 + lane < each && r < n;
-        values[i] = there ? a.row_values[at + r] : nothing;
-      }
-    };
-    if constexpr (kKeysPass) load_values(0);
     for (int t = 0; t < nt; ++t) {
-      const int stage = t % S::kStages;
-      const int at = (begin + t) * each;
-      const uint32_t t1 = y1 + stage * S::kTile, t2 = y2 + stage * S::kTile;
-      uint32_t open[W / 32];
-      bool whole;
-      if constexpr (kKeysPass) {
-        key_words<W>(open, nullptr, 0, min(n - at, each));
-        whole = n - at >= each;
-      } else {
-        key_words<W>(open, mask, at, nk);
-        whole = true;
-#pragma unroll
-        for (int i = 0; i < W / 32; ++i) whole &= open[i] == 0xffffffffu;
-      }
-      if (t >= S::kStages) wait(kTileFree + stage, t / S::kStages - 1);
-      const int full = whole ? kTileFull + stage : kTileRaw;
-      __syncwarp();
-      if (tc::elect()) {
-        tc::barrier_expect(bar(full), 2 * panels * each * 128);
-        const int head = kKeysPass ? hk * a.group : hk;
-        const int row = kKeysPass ? q0 + at / a.group : k0 + at;
-        for (int p = 0; p < panels; ++p) {
-          tc::copy_box(t1 + p * W * 128, &maps.y1, bar(full), p * 64, head,
-                       row);
-          tc::copy_box(t2 + p * W * 128, &maps.y2, bar(full), p * 64, head,
-                       row);
-        }
-      }
-      if constexpr (kKeysPass) {
-#pragma unroll
-        for (int i = 0; i < W / 32; ++i) {
-          const uint32_t to =
-              stage * S::kTileMore + tc::narrow_offset(i * 32 + lane, 0);
-          store(y1_more + to, values[i].x, values[i].y);
-          store(y2_more + to, values[i].z, values[i].w);
-        }
-        load_values(t + 1);
-      }
-      if (!whole) {
-        wait(kTileRaw, cleared++);
-        __syncwarp();
-        clear_rows<W>(t1, panels, open);
-        if constexpr (kKeysPass) clear_rows<W>(t2, panels, open);
-      }
-      if (!whole || kKeysPass) {
-        tc::fence_shared();
-        __syncwarp();
-        // in the keys' pass a tile is there with its copies and its values
-        if (lane == 0) {
-          tc::barrier_arrive(bar(kTileFull + stage));
-          if (!whole && kKeysPass) tc::barrier_arrive(bar(kTileFull + stage));
-        }
-      }
+      if (t >= S::kStages) issue(t);
+      finish(t);
     }
   } else if (warp == kRowWarps) {
     for (int t = 0; t < nt; ++t) {

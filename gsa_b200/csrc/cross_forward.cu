@@ -62,12 +62,12 @@ enum Bar {
   kKeysFree = 2,    // [stage] the scores that read them are complete
   kValuesFull = 4,  // [stage]
   kValuesFree = 6,  // [stage]
-  kValuesRaw = 8,   // values loaded, rows to be cleared
-  kScores = 9,      // S is complete
-  kScoresRead = 10,  // S is in registers (a count per warp of rows)
-  kWeights = 11,    // P is there (a count per warp of rows)
-  kOutput = 12,     // O += P V is complete
-  kBars = 13
+  kValuesRaw = 8,   // [stage] values loaded, rows to be cleared
+  kScores = 10,     // S is complete
+  kScoresRead = 11,  // S is in registers (a count per warp of rows)
+  kWeights = 12,    // P is there (a count per warp of rows)
+  kOutput = 13,     // O += P V is complete
+  kBars = 14
 };
 
 // The largest of three, NaN if one is.
@@ -113,15 +113,63 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto wait = [&](int which, int phase) {
     if (ok) ok = tc::barrier_wait(bar0 + which * 8, phase & 1);
   };
+  // The loading warp: a tile's copies, and what is left to do when they are
+  // there.
+  const int panels = a.dim > 64 ? 2 : 1;
+  int cleared = 0;  // a bit per stage: the phase of its raw barrier
+  auto whole = [&](int t, uint32_t* open) {
+    key_words<kKeys>(open, mask, (begin + t) * kKeys, nk);
+    return (open[0] & open[1] & open[2] & open[3]) == 0xffffffffu;
+  };
+  auto issue = [&](int t) {
+    const int stage = t % S::kStages, round = t / S::kStages;
+    const int at = k0 + (begin + t) * kKeys;
+    uint32_t open[kKeys / 32];
+    const int full = (whole(t, open) ? kValuesFull : kValuesRaw) + stage;
+    if (round > 0) wait(kKeysFree + stage, round - 1);
+    __syncwarp();
+    if (tc::elect()) {
+      tc::barrier_expect(bar(kKeysFull + stage), panels * kKeys * 128);
+      for (int p = 0; p < panels; ++p)
+        tc::copy_box(k_tile + stage * S::kTile + p * kKeys * 128, &maps.k,
+                     bar(kKeysFull + stage), p * 64, hk, at);
+    }
+    if (round > 0) wait(kValuesFree + stage, round - 1);
+    __syncwarp();
+    if (tc::elect()) {
+      tc::barrier_expect(bar(full), panels * kKeys * 128);
+      for (int p = 0; p < panels; ++p)
+        tc::copy_box(v_tile + stage * S::kTile + p * kKeys * 128, &maps.v,
+                     bar(full), p * 64, hk, at);
+    }
+    __syncwarp();
+  };
+  auto finish = [&](int t) {
+    const int stage = t % S::kStages;
+    uint32_t open[kKeys / 32];
+    if (whole(t, open)) return;
+    wait(kValuesRaw + stage, cleared >> stage);
+    cleared ^= 1 << stage;
+    __syncwarp();
+    clear_rows<kKeys>(v_tile + stage * S::kTile, panels, open);
+    tc::fence_shared();
+    __syncwarp();
+    if (lane == 0) tc::barrier_arrive(bar(kValuesFull + stage));
+  };
+
   if (nt > 0) {
     if (warp == 4) {
       tc::tmem_alloc(tc::smem_address(&tmem_at), S::kColumns);
+    } else if (warp == 5) {
       if (lane == 0) {
         for (int i = 0; i < kBars; ++i)
           tc::barrier_init(bar(i), i == kScoresRead || i == kWeights ? 4 : 1);
         tc::barriers_ready();
       }
-    } else if (warp < 4) {
+      __syncwarp();
+      // the first tiles come while the block gets ready
+      for (int t = 0; t < S::kStages && t < nt; ++t) issue(t);
+    } else {
       load_packed<T, kRows>(
           chunks_of(a.dim, tid, kRows), q_tile,
           static_cast<const T*>(a.q) + q0 * a.q_row +
@@ -138,42 +186,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   if (warp == 5) {
-    const int panels = a.dim > 64 ? 2 : 1;
-    int cleared = 0;
     for (int t = 0; t < nt; ++t) {
-      const int stage = t % S::kStages, round = t / S::kStages;
-      const int at = (begin + t) * kKeys;
-      const uint32_t kt = k_tile + stage * S::kTile,
-                     vt = v_tile + stage * S::kTile;
-      uint32_t open[kKeys / 32];
-      key_words<kKeys>(open, mask, at, nk);
-      const bool whole =
-          (open[0] & open[1] & open[2] & open[3]) == 0xffffffffu;
-      const int full = whole ? kValuesFull + stage : kValuesRaw;
-      if (round > 0) wait(kKeysFree + stage, round - 1);
-      __syncwarp();
-      if (tc::elect()) {
-        tc::barrier_expect(bar(kKeysFull + stage), panels * kKeys * 128);
-        for (int p = 0; p < panels; ++p)
-          tc::copy_box(kt + p * kKeys * 128, &maps.k, bar(kKeysFull + stage),
-                       p * 64, hk, k0 + at);
-      }
-      if (round > 0) wait(kValuesFree + stage, round - 1);
-      __syncwarp();
-      if (tc::elect()) {
-        tc::barrier_expect(bar(full), panels * kKeys * 128);
-        for (int p = 0; p < panels; ++p)
-          tc::copy_box(vt + p * kKeys * 128, &maps.v, bar(full), p * 64, hk,
-                       k0 + at);
-      }
-      if (!whole) {
-        wait(kValuesRaw, cleared++);
-        __syncwarp();
-        clear_rows<kKeys>(vt, panels, open);
-        tc::fence_shared();
-        __syncwarp();
-        if (lane == 0) tc::barrier_arrive(bar(kValuesFull + stage));
-      }
+      if (t >= S::kStages) issue(t);
+      finish(t);
     }
   } else if (warp == 4) {
     const int steps = (a.dim + 15) / 16;
@@ -399,13 +414,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// The parts of a split row, joined: a warp per (row, head).
+// The parts of a split row, joined: a block per (row, head), whose warps take
+// the parts in turn.
 template <typename T>
 __global__ void __launch_bounds__(128)
     cross_join_kernel(const __grid_constant__ CrossArgs a) {
-  const long long unit = ((long long)blockIdx.x * 128 + threadIdx.x) >> 5;
-  if (unit >= a.n_q * a.heads) return;
-  const int lane = threadIdx.x & 31;
+  __shared__ float4 sums[4][32];
+  __shared__ float weights[4];
+  const long long unit = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long step = a.n_q * a.heads;
   float top = -kInf;
   bool nan = false;
@@ -421,7 +438,8 @@ __global__ void __launch_bounds__(128)
   float sum = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
   const bool mine = lane * 4 < a.dim;
   if (top != -kInf) {
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += 4) {
       const float w = exp2_fast(a.part_lse[s * step + unit] - top);
       sum += w;
       if (mine) {
@@ -433,9 +451,20 @@ __global__ void __launch_bounds__(128)
         f[3] = fmaf(w, x.w, f[3]);
       }
     }
-    const float inv = 1.f / sum;
+  }
+  sums[warp][lane] = make_float4(f[0], f[1], f[2], f[3]);
+  if (lane == 0) weights[warp] = sum;
+  __syncthreads();
+  if (warp > 0) return;
+  sum = (weights[0] + weights[1]) + (weights[2] + weights[3]);
+  const float inv = top == -kInf ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] *= inv;
+  for (int i = 0; i < 4; ++i) {
+    f[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      f[i] += reinterpret_cast<const float*>(&sums[w][lane])[i];
+    f[i] *= inv;
   }
   if (nan) {
 #pragma unroll
@@ -467,7 +496,7 @@ cudaError_t launch(const CrossArgs& a, const Maps& maps, long long units,
   if (a.splits > 1) {
     count_launches(1);
     cross_join_kernel<T>
-        <<<(unsigned)ceil_div(a.n_q * a.heads, 4), 128, 0, s>>>(a);
+        <<<(unsigned)(a.n_q * a.heads), 128, 0, s>>>(a);
   }
   return cudaGetLastError();
 }
@@ -485,13 +514,22 @@ int multiprocessors() {
   return n;
 }
 
-// How many blocks share a row of work: as many as still find room on the GPU
-// together, each with at least two tiles.
+// How many blocks share a row of work: what takes the least time, in tiles, if
+// a block costs five of them to begin and end, `room` blocks run together, and
+// parts cost ten more to be joined.
 int split_count(long long blocks, long long tiles, int room) {
-  if (blocks < 1 || tiles < 4) return 1;
-  long long n = room / blocks;
-  if (n > tiles / 2) n = tiles / 2;
-  return n < 1 ? 1 : (int)n;
+  if (blocks < 1 || blocks >= 8ll * room) return 1;
+  int best = 1;
+  long long least = ceil_div(blocks, room) * (tiles + 5);
+  for (int n = 2; n <= 128 && 2 * n <= tiles; ++n) {
+    const long long t =
+        ceil_div(blocks * n, room) * (ceil_div(tiles, n) + 5) + 10;
+    if (t < least) {
+      least = t;
+      best = n;
+    }
+  }
+  return best;
 }
 
 bool cross_sizes(const attention_args* a) {

@@ -62,6 +62,17 @@ __global__ void __launch_bounds__(32 * kWarps)
       ((long long)blockIdx.x * kWarps + warp) * per_warp + group;
   const bool live = group < per_warp && row < a.rows;
   const int half = a.axes * a.pairs, part = 2 * half;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_row + j * V;
+  T* y = static_cast<T*>(a.y) + row * a.y_row + j * V;
+  // the first heads' rows are on their way while the sines are taken
+  uint4 u[kHeadsAhead];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int k = 0; k < kHeadsAhead; ++k)
+      if (live && h0 + k < a.heads)
+        u[k] = *reinterpret_cast<const uint4*>(x + (h0 + k) * a.x_head);
+  };
+  load(0);
   float c[V], s[V];
   if (live) {
     if constexpr (kInterleaved) {
@@ -86,14 +97,8 @@ __global__ void __launch_bounds__(32 * kWarps)
       }
     }
   }
-  const T* x = static_cast<const T*>(a.x) + row * a.x_row + j * V;
-  T* y = static_cast<T*>(a.y) + row * a.y_row + j * V;
   for (int h0 = 0; h0 < a.heads; h0 += kHeadsAhead) {
-    uint4 u[kHeadsAhead];
-#pragma unroll
-    for (int k = 0; k < kHeadsAhead; ++k)
-      if (live && h0 + k < a.heads)
-        u[k] = *reinterpret_cast<const uint4*>(x + (h0 + k) * a.x_head);
+    if (h0 > 0) load(h0);
     if constexpr (!kInterleaved) {
 #pragma unroll
       for (int k = 0; k < kHeadsAhead; ++k)

@@ -31,8 +31,11 @@ __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
                "r"(bytes)
                : "memory");
 }
+// The barriers that this thread initialised, visible to the block's threads
+// (after a barrier of theirs) and to copies and products.
 __device__ __forceinline__ void barriers_ready() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
 // Every wait is for work of the same block that is under way and takes
