@@ -100,6 +100,34 @@ struct Pairs {
   }
 };
 
+// The products of two words' 16-bit elements, added to 32 bits without being
+// unpacked.
+template <typename T>
+__device__ __forceinline__ float fma_word(uint32_t a, uint32_t b, float c) {
+  if constexpr (__is_same(T, __nv_bfloat16))
+    asm("{\n .reg .b16 a0, a1, b0, b1;\n mov.b32 {a0, a1}, %1;\n"
+        " mov.b32 {b0, b1}, %2;\n fma.rn.f32.bf16 %0, a0, b0, %0;\n"
+        " fma.rn.f32.bf16 %0, a1, b1, %0;\n}\n"
+        : "+f"(c)
+        : "r"(a), "r"(b));
+  else
+    asm("{\n .reg .b16 a0, a1, b0, b1;\n mov.b32 {a0, a1}, %1;\n"
+        " mov.b32 {b0, b1}, %2;\n fma.rn.f32.f16 %0, a0, b0, %0;\n"
+        " fma.rn.f32.f16 %0, a1, b1, %0;\n}\n"
+        : "+f"(c)
+        : "r"(a), "r"(b));
+  return c;
+}
+template <typename T>
+__device__ __forceinline__ float dot(const uint4& a, const uint4& b) {
+  if constexpr (sizeof(T) == 4) {
+    return Pairs<T>(a).dot(Pairs<T>(b));
+  } else {
+    return fma_word<T>(a.x, b.x, fma_word<T>(a.z, b.z, 0.f)) +
+           fma_word<T>(a.y, b.y, fma_word<T>(a.w, b.w, 0.f));
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 vector_at(const void* base, long long element) {
   return __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) +
@@ -193,12 +221,11 @@ __global__ void __launch_bounds__(kBlock)
     neighbor_forward_kernel(const __grid_constant__ NeighborArgs a) {
   __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
   const Group<T, L> g(a, lists);
-  Pairs<T> q, acc;
-  q.clear();
+  Pairs<T> acc;
   acc.clear();
+  uint4 q = make_uint4(0, 0, 0, 0);
   if (g.mine)
-    q = Pairs<T>(vector_at<T>(a.q, g.row * a.q_row + g.h * a.q_head +
-                                       g.j * Vec<T>::V));
+    q = vector_at<T>(a.q, g.row * a.q_row + g.h * a.q_head + g.j * Vec<T>::V);
   float m = -kInf, l = 0.f;
   for (int j0 = 0; __any_sync(kFull, j0 < g.n); j0 += kAhead) {
     uint4 ku[kAhead], vu[kAhead];
@@ -206,7 +233,7 @@ __global__ void __launch_bounds__(kBlock)
     float s[kAhead], top = m;
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      s[t] = group_sum<L>(Pairs<T>(ku[t]).dot(q)) * a.scale_log2e;
+      s[t] = group_sum<L>(dot<T>(ku[t], q)) * a.scale_log2e;
       if (j0 + t >= g.n) s[t] = -kInf;
       top = fmaxf(top, s[t]);
     }
@@ -240,16 +267,15 @@ __global__ void __launch_bounds__(kBlock)
   __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
   const Group<T, L> g(a, lists);
   const int at = g.j * Vec<T>::V;
-  Pairs<T> q, d, acc;
-  q.clear();
-  d.clear();
+  Pairs<T> acc;
   acc.clear();
+  uint4 q = make_uint4(0, 0, 0, 0), d = q;
   float part = 0.f;
   if (g.mine) {
-    q = Pairs<T>(vector_at<T>(a.q, g.row * a.q_row + g.h * a.q_head + at));
-    d = Pairs<T>(vector_at<T>(a.dout, g.row * a.d_row + g.h * a.d_head + at));
-    part = Pairs<T>(vector_at<T>(a.out, g.row * a.o_row + g.h * a.o_head + at))
-               .dot(d);
+    q = vector_at<T>(a.q, g.row * a.q_row + g.h * a.q_head + at);
+    d = vector_at<T>(a.dout, g.row * a.d_row + g.h * a.d_head + at);
+    part = dot<T>(
+        vector_at<T>(a.out, g.row * a.o_row + g.h * a.o_head + at), d);
   }
   const float delta = group_sum<L>(part);
   if (g.live && g.j == 0) a.delta[g.unit] = delta;
@@ -259,11 +285,10 @@ __global__ void __launch_bounds__(kBlock)
     g.load(a, j0, ku, vu);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      const Pairs<T> k(ku[t]);
-      const float s = group_sum<L>(k.dot(q));
-      const float dp = group_sum<L>(Pairs<T>(vu[t]).dot(d));
+      const float s = group_sum<L>(dot<T>(ku[t], q));
+      const float dp = group_sum<L>(dot<T>(vu[t], d));
       const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2));
-      if (j0 + t < g.n) acc.add(p * (dp - delta), k);
+      if (j0 + t < g.n) acc.add(p * (dp - delta), Pairs<T>(ku[t]));
     }
   }
   if (g.mine) {
@@ -290,14 +315,13 @@ __global__ void __launch_bounds__(kBlock, 8)
   const long long key = unit / a.kv_heads;
   const int hk = (int)(unit - key * a.kv_heads);
   const bool mine = j * V < a.dim;
-  Pairs<T> k, v, dk, dv;
-  k.clear();
-  v.clear();
+  Pairs<T> dk, dv;
   dk.clear();
   dv.clear();
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
   if (mine) {
-    k = Pairs<T>(vector_at<T>(a.k, key * a.k_row + hk * a.k_head + j * V));
-    v = Pairs<T>(vector_at<T>(a.v, key * a.v_row + hk * a.v_head + j * V));
+    k = vector_at<T>(a.k, key * a.k_row + hk * a.k_head + j * V);
+    v = vector_at<T>(a.v, key * a.v_row + hk * a.v_head + j * V);
   }
   const int from = __ldg(a.starts + key), to = __ldg(a.starts + key + 1);
   for (int e0 = from; e0 < to; e0 += 32) {
@@ -328,12 +352,12 @@ __global__ void __launch_bounds__(kBlock, 8)
         }
 #pragma unroll
         for (int t = 0; t < kDeep; ++t) {
-          const Pairs<T> q(qu[t]), d(du[t]);
-          const float s = group_sum<L>(q.dot(k)), dp = group_sum<L>(d.dot(v));
+          const float s = group_sum<L>(dot<T>(qu[t], k));
+          const float dp = group_sum<L>(dot<T>(du[t], v));
           if (t0 + t * G + who >= n) continue;
           const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2[t]));
-          dk.add(p * (dp - delta[t]), q);
-          dv.add(p, d);
+          dk.add(p * (dp - delta[t]), Pairs<T>(qu[t]));
+          dv.add(p, Pairs<T>(du[t]));
         }
       }
     }
