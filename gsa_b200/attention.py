@@ -67,7 +67,7 @@ class _Call:
     """The checked arguments that one attention call and its gradient share."""
 
     __slots__ = ("what", "device", "stream", "pairs", "dtype", "q_shape", "k_shape", "on", "sizes", "rows", "mask", "ids",
-                 "width", "padded")
+                 "width", "padded", "copies")
 
     def __init__(self, what, q, k, v, pairs, scale, types):
         try:
@@ -95,12 +95,20 @@ class _Call:
         self.what, self.dtype, self.pairs, self.on = what, q.dtype, pairs, q.device
         self.q_shape, self.k_shape = (n_q, heads, dim), (n_k, kv_heads, dim)
         self.sizes = (ft.TYPES[q.dtype], pairs.scenes, n_q, n_k, pairs.max_q, pairs.max_k, heads, kv_heads, dim, scale)
+        self.copies = [] if types is _HALF else None
         self.rows = self.rows_of(q, "q", self.q_shape) + self.rows_of(k, "k", self.k_shape) + self.rows_of(
             v, "v", self.k_shape)
         self.mask = self.ids = self.width = self.padded = 0
 
     def rows_of(self, t, name, shape):
-        return ft.vector_rows_of(t, name, shape, self.dtype, self.device)
+        found = ft.vector_rows_of(t, name, shape, self.dtype, self.device)
+        if self.copies is not None and ((not found[1] and shape[0] > 1) or (not found[2] and shape[1] > 1)):
+            # expanded rows or heads: the cross-attention kernels' copy engine
+            # takes no stride of 0
+            t = t.contiguous()
+            self.copies.append(t)
+            found = ft.vector_rows_of(t, name, shape, self.dtype, self.device)
+        return found
 
     def set_mask(self, mask):
         if mask is None:
@@ -176,7 +184,11 @@ _ALL = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _wants_grad(out, *tensors):
-    return out is None and any(getattr(t, "requires_grad", False) for t in tensors) and torch.is_grad_enabled()
+    if not (any(getattr(t, "requires_grad", False) for t in tensors) and torch.is_grad_enabled()):
+        return False
+    if out is not None:
+        raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
+    return True
 
 
 def _cross(q, k, v, pairs, mask, scale, out, return_lse):
@@ -195,9 +207,12 @@ def cross_attention(q, k, v, pairs, mask=None, scale=None, out=None, return_lse=
     and head strides are free in steps of 16 bytes.  ``mask``: bool (N_k,),
     False shuts a key out, whatever it holds.  ``scale``: dim ** -0.5 by
     default, from 2^-24 to 2^24.  A query without open keys gets 0.  Returns ``out`` (written to
-    ``out`` if given), and with ``return_lse`` also the FP32 (N_q, heads)
-    logarithms of the sums of exponentials that ``cross_attention_grad``
-    takes.  Without ``out``, differentiable in q, k and v."""
+    ``out`` if given, which does not overlap the inputs), and with
+    ``return_lse`` also the FP32 (N_q, heads) logarithms of the sums of
+    exponentials that ``cross_attention_grad`` takes.  Differentiable in q, k
+    and v unless ``out`` is given.  In a captured graph, take the gradient by
+    ``cross_attention_grad``: torch's autograd may order a captured backward
+    pass after work outside the capture."""
     if _wants_grad(out, q, k, v):
         out, lse = _Cross.apply(q, k, v, pairs, mask, scale)
         return (out, lse) if return_lse else out

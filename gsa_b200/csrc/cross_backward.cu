@@ -87,29 +87,30 @@ enum Bar {
 
 // Factors that P and dS carry (2^x).
 template <typename T>
-__device__ __forceinline__ float p_bits() {
-  return __is_same(T, __half) ? 15.f : 0.f;
+__device__ __forceinline__ int p_bits() {
+  return __is_same(T, __half) ? 15 : 0;
 }
 template <typename T>
-__device__ __forceinline__ float ds_bits(int keys) {
-  if (!__is_same(T, __half)) return 0.f;
+__device__ __forceinline__ int ds_bits(int keys) {
   const int b = 31 - __clz(keys | 1) - 10;
-  return b > 0 ? (float)b : 0.f;
+  return __is_same(T, __half) && b > 0 ? b : 0;
+}
+__device__ __forceinline__ float power_of_two(int e) {  // -126 to 127
+  return __int_as_float((127 + e) << 23);
 }
 
 // x as three values of T that stand for multiples of 2^e, 2^(e-8) and
-// 2^(e-19): the exponents keep fp16 from overflowing (x below 2^(e+16)) and
-// from losing what lies below its normals.
+// 2^(e-19): the exponents keep fp16 from overflowing (x below 2^(e+16), what
+// is beyond gives NaN) and from losing what lies below its normals.
 template <typename T>
 __device__ __forceinline__ uint2 three_parts(float x, int e) {
-  const float f0 = exp2f((float)e), f1 = exp2f((float)(e - 8)),
-              f2 = exp2f((float)(e - 19));
-  const float h = to_float(from_float<T>(x / f0));
-  float m = 0.f, l = 0.f;
+  float h = to_float(from_float<T>(x * power_of_two(-e))), m = 0.f, l = 0.f;
   if (fabsf(h) < kInf) {
-    const float r = x - h * f0;
-    m = to_float(from_float<T>(r / f1));
-    l = (r - m * f1) / f2;
+    const float r = x - h * power_of_two(e);
+    m = to_float(from_float<T>(r * power_of_two(8 - e)));
+    l = (r - m * power_of_two(e - 8)) * power_of_two(19 - e);
+  } else if (fabsf(x) < kInf) {
+    h = __int_as_float(0x7fffffff);
   }
   return make_uint2(pack2<T>(h, m), pack2<T>(l, 0.f));
 }
@@ -122,7 +123,8 @@ __device__ __forceinline__ void product_more(uint32_t d, uint32_t a,
           tc::instruction<T>(kN, false), true);
 }
 
-template <typename T, int kDim, bool kKeysPass>
+// kOneTile: no scene has more walked rows than a tile (queries' pass).
+template <typename T, int kDim, bool kKeysPass, bool kOneTile>
 __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
                                   Shape<kDim, kKeysPass>::kBlocks)
     cross_backward_kernel(const __grid_constant__ CrossArgs a,
@@ -174,8 +176,8 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
                  "r"(u1), "r"(0)
                  : "memory");
   };
-  const float bits = ds_bits<T>(nk);
-  const float ds_factor = exp2f(bits - p_bits<T>());
+  const int bits = ds_bits<T>(nk);
+  const float ds_factor = power_of_two(bits - p_bits<T>());
   // the exponents of the further columns' first part: of lse / scale, so that
   // lse is below 2^16; of delta
   const int s_exp = a.scale_exponent, d_exp = 8;
@@ -297,8 +299,8 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
             const int e = x ? d_exp : s_exp;
             const uint32_t to = x ? x2_more : x1_more;
             store(to + tc::narrow_offset(tid, 0),
-                  pack2<T>(exp2f((float)e), exp2f((float)(e - 8))),
-                  pack2<T>(exp2f((float)(e - 19)), 0.f));
+                  pack2<T>(power_of_two(e), power_of_two(e - 8)),
+                  pack2<T>(power_of_two(e - 19), 0.f));
             store(to + tc::narrow_offset(tid, 1), 0, 0);
           }
         }
@@ -306,7 +308,8 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
           for (int s = 0; s < 2 * S::kStages; ++s)
             store(y1_more + s * S::kTileMore + tc::narrow_offset(tid, 1), 0, 0);
       } else {
-        // delta = <dout, out>, a share of the row's elements each
+        // delta = <dout, out>, a share of the row's elements each (of one
+        // tile it comes from P and dP instead)
         const int r = min(r0 + (tid & (kRows - 1)), n - 1), qr = r / a.group;
         const int h = hk * a.group + r - qr * a.group;
         const T* o = static_cast<const T*>(a.out) + (q0 + qr) * a.o_row +
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         for (int i = 0; i < kEach; ++i) {
           const int at = ((tid >> 7) + i * S::kShare) * 8;
           u[i] = v[i] = make_uint4(0, 0, 0, 0);
-          if (at < a.dim) {
+          if (!kOneTile && at < a.dim) {
             u[i] = *reinterpret_cast<const uint4*>(o + at);
             v[i] = *reinterpret_cast<const uint4*>(d + at);
           }
@@ -406,25 +409,36 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
     const uint32_t mine = tmem + ((uint32_t)group << 21);
     bool open = live;
     float lse2 = -kInf, delta = 0.f;
+    // what the keys' pass needs of this row
+    auto put_values = [&](float minus_delta) {
+      const uint2 u = three_parts<T>(lse2 / a.scale_log2e, s_exp);
+      const uint2 v = three_parts<T>(minus_delta, d_exp);
+      a.row_values[((long long)hk * a.n_q + q0) * a.group + r] =
+          make_uint4(u.x, u.y, v.x, v.y);
+    };
+    auto my_word = [&](const uint32_t* words) {  // of this thread's columns
+      uint32_t word = words[0];
+#pragma unroll
+      for (int i = 1; i < W / 32; ++i)
+        if (part == i) word = words[i];
+      return word;
+    };
     if constexpr (kKeysPass) {
       open = live && (!mask || __ldg(mask + r));
     } else if (nt > 0) {
+      if constexpr (!kOneTile) {
 #pragma unroll
-      for (int i = 0; i < S::kShare; ++i)
-        delta += part_delta[i][group * 32 + lane];
+        for (int i = 0; i < S::kShare; ++i)
+          delta += part_delta[i][group * 32 + lane];
+      }
       if (live) {
         const int qr = r / a.group;
         const long long row = q0 + qr;
         const int h = hk * a.group + (r - qr * a.group);
         // a row without keys gets P = 0
         const float x = __ldg(a.lse + row * a.heads + h);
-        if (x != -kInf) lse2 = fmaf(x, -kLog2e, p_bits<T>());
-        if (part == 0) {
-          const long long e = ((long long)hk * a.n_q + q0) * a.group + r;
-          const uint2 u = three_parts<T>(lse2 / a.scale_log2e, s_exp);
-          const uint2 v = three_parts<T>(-delta, d_exp);
-          a.row_values[e] = make_uint4(u.x, u.y, v.x, v.y);
-        }
+        if (x != -kInf) lse2 = fmaf(x, -kLog2e, (float)p_bits<T>());
+        if (!kOneTile && part == 0) put_values(-delta);
       }
       delta *= -ds_factor;
     }
@@ -433,7 +447,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
     const uint64_t scale2 = tc::pair(a.scale_log2e, a.scale_log2e);
     const uint64_t factor2 = tc::pair(ds_factor, ds_factor);
     const uint64_t row_lse2 = tc::pair(lse2, lse2);
-    const uint64_t row_delta2 = tc::pair(delta, delta);
+    uint64_t row_delta2 = tc::pair(delta, delta);
     if (!busy) {
       for (int t = 0; t < nt; ++t) {
         wait(kScores, t);
@@ -462,6 +476,35 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         tc::fence_before();
         __syncwarp();
         if (lane == 0) tc::barrier_arrive(bar(kRead));
+        uint32_t words[W / 32];
+        bool some = false;  // keys of the tile are shut or absent
+        if constexpr (!kKeysPass) {
+          const int first = (begin + t) * W;
+          some = mask || first + W > nk;
+          if (some) key_words<W>(words, mask, first, nk);
+          if constexpr (kOneTile) {
+            // All keys are here: delta is the sum of P * dP, without the
+            // rounding of `out` (of few keys its largest error).
+            float sum = 0.f;
+            const uint32_t word = some ? my_word(words) : 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              const float w = exp2_fast(
+                  fmaf(__uint_as_float(s[i]), a.scale_log2e, lse2));
+              if ((word >> i) & 1) sum = fmaf(w, __uint_as_float(d[i]), sum);
+            }
+            part_delta[part][group * 32 + lane] = sum;
+            __syncwarp();
+            tc::meet(1 + group, 32 * S::kShare);
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::kShare; ++i)
+              sum += part_delta[i][group * 32 + lane];
+            sum *= power_of_two(-p_bits<T>());
+            row_delta2 = tc::pair(-sum * ds_factor, -sum * ds_factor);
+            if (live && part == 0) put_values(-sum);
+          }
+        }
         uint32_t p[kMine / 2], ds[kMine / 2];
 #pragma unroll
         for (int i = 0; i < kMine; i += 2) {
@@ -493,14 +536,8 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
             }
           }
         } else {
-          const int first = (begin + t) * W;
-          if (mask || first + W > nk) {
-            uint32_t words[W / 32];
-            key_words<W>(words, mask, first, nk);
-            uint32_t word = words[0];  // of this thread's 32 columns
-#pragma unroll
-            for (int i = 1; i < W / 32; ++i)
-              if (part == i) word = words[i];
+          if (some) {
+            const uint32_t word = my_word(words);
 #pragma unroll
             for (int i = 0; i < kMine / 2; ++i) {
               const uint32_t two = word >> (2 * i);
@@ -547,7 +584,8 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
       }
 #pragma unroll
       for (int which = 0; which < (kKeysPass ? 2 : 1); ++which) {
-        const float f = which ? exp2f(-p_bits<T>()) : a.scale * exp2f(-bits);
+        const float f = which ? power_of_two(-p_bits<T>())
+                              : a.scale * power_of_two(-bits);
         T* out = static_cast<T*>(kKeysPass ? (which ? a.dv : a.dk) : a.dq) + at;
         float* sum = a.part + ((kKeysPass ? 2 : 1) * split + which) * parts + at;
         for (int i = part * 8; i < a.dim; i += 8 * S::kShare) {
@@ -637,7 +675,7 @@ Plan backward_plan(const attention_args* a) {
   return p;
 }
 
-template <typename T, int kDim, bool kKeysPass>
+template <typename T, int kDim, bool kKeysPass, bool kOneTile>
 cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
                         cudaStream_t s) {
   using S = Shape<kDim, kKeysPass>;
@@ -661,12 +699,12 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
                   S::kWalk);
   }
   if (!e)
-    e = cudaFuncSetAttribute(cross_backward_kernel<T, kDim, kKeysPass>,
+    e = cudaFuncSetAttribute(cross_backward_kernel<T, kDim, kKeysPass, kOneTile>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                            S::kSmem);
   if (e) return e;
   count_launches(1);
-  cross_backward_kernel<T, kDim, kKeysPass>
+  cross_backward_kernel<T, kDim, kKeysPass, kOneTile>
       <<<(unsigned)grid, S::kThreads, S::kSmem, s>>>(a, maps);
   if (a.splits > 1) {
     const long long n =
@@ -690,11 +728,18 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
 template <typename T>
 cudaError_t launch(const CrossArgs& a, const attention_args* in, const Plan& p,
                    cudaStream_t s) {
-  cudaError_t e = a.dim <= 64 ? launch_pass<T, 64, false>(a, in, p, s)
-                              : launch_pass<T, 128, false>(a, in, p, s);
+  cudaError_t e;
+  if (a.dim <= 64)
+    e = in->max_k <= Shape<64, false>::kWalk
+            ? launch_pass<T, 64, false, true>(a, in, p, s)
+            : launch_pass<T, 64, false, false>(a, in, p, s);
+  else
+    e = in->max_k <= Shape<128, false>::kWalk
+            ? launch_pass<T, 128, false, true>(a, in, p, s)
+            : launch_pass<T, 128, false, false>(a, in, p, s);
   if (e) return e;
-  return a.dim <= 64 ? launch_pass<T, 64, true>(a, in, p, s)
-                     : launch_pass<T, 128, true>(a, in, p, s);
+  return a.dim <= 64 ? launch_pass<T, 64, true, false>(a, in, p, s)
+                     : launch_pass<T, 128, true, false>(a, in, p, s);
 }
 
 }  // namespace

@@ -59,6 +59,12 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
   return left != 0;
 }
 
+// Some warps of a block meet: `threads` of them in all, by a number of their
+// own (1 to 15).
+__device__ __forceinline__ void meet(int number, int threads) {
+  asm volatile("barrier.sync %0, %1;" ::"r"(number), "r"(threads) : "memory");
+}
+
 // ---- tensor memory --------------------------------------------------------
 
 // By one whole warp; columns: a power of two of at least 32.

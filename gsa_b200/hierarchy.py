@@ -158,6 +158,17 @@ class Batch:
         z["snapshot"] = torch.empty((B, self.sizes[0], 3), device=device)
         return z
 
+    def pairs(self, B, s, t):
+        """``ScenePairs`` of ``B`` scenes whose queries are the points of
+        level ``s`` and whose keys are those of level ``t`` (features packed
+        scene after scene, ``B * sizes[s]`` and ``B * sizes[t]`` rows): what
+        ``cross_attention`` between the levels takes, and, for s = t,
+        ``neighbor_attention`` along the rows ``ball<s>``; ``hit<s>`` are rows
+        of ``pairs(B, s + 1, s)``."""
+        from .attention import ScenePairs
+
+        return ScenePairs.of_lengths([self.sizes[s]] * B, [self.sizes[t]] * B)
+
     def _side_streams(self, device):
         streams = self._streams.get(device)
         if streams is None:

@@ -119,8 +119,10 @@ class Rotary:
         """The rows ``x`` (FP32, FP16 or BF16 (N, heads, dim), any row and
         head strides) turned by ``positions`` (FP32, int32 or int64
         (N, axes), or (N,) for one axis).  ``out`` may be ``x`` itself, else it does not
-        overlap it.  Differentiable in ``x`` when ``out`` is not given."""
-        if out is None and getattr(x, "requires_grad", False) and torch.is_grad_enabled():
+        overlap it.  Differentiable in ``x`` unless ``out`` is given."""
+        if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
+            if out is not None:
+                raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
             return _Turn.apply(x, positions, self)
         return self._run(x, positions, out, False)
 

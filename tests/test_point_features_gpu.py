@@ -493,6 +493,104 @@ def test_streams_and_captured_graphs(kind):
         assert all(torch.equal(a, b) for a, b in zip(got, (out, lse, *want)))
 
 
+def test_expanded_inputs_and_gradients():
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(170, ([70, 3], [200, 60]), 4, 4, 32, BF16)
+    pairs = ScenePairs(q_seg, k_seg)
+    one = [q[:1].expand(73, 4, 32), k[:, :1].expand(260, 4, 32), v[:1, :1].expand(260, 4, 32)]
+    d = normal(171, 1, 1, 32, dtype=BF16).expand(73, 4, 32)
+    same = [t.contiguous() for t in one]
+    out, lse = cross_attention(*one, pairs, return_lse=True)
+    assert torch.equal(out, cross_attention(*same, pairs))
+    got = cross_attention_grad(d, *one, out, lse, pairs)
+    assert all(torch.equal(a, b) for a, b in zip(got, cross_attention_grad(d.contiguous(), *same, out, lse, pairs)))
+    # broadcast leaves get their sums
+    leaf = k[:, :1].clone().requires_grad_()
+    cross_attention(q, leaf.expand(260, 4, 32), v, pairs).backward(same[0])
+    whole = k[:, :1].expand(260, 4, 32).clone().requires_grad_()
+    cross_attention(q, whole, v, pairs).backward(same[0])
+    assert torch.equal(leaf.grad, whole.grad.sum(1, keepdim=True))
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (32, FP16), (128, BF16)])
+@pytest.mark.parametrize("n_k", [1, 2, 5, 64])
+def test_cross_gradients_of_few_keys(n_k, dim, dtype):
+    # keys of one tile: delta comes from P and dP, not from the output
+    q, k, v, q_seg, k_seg = attention_inputs(180, ([130], [n_k]), 2, 1, dim, dtype)
+    want = check_cross(q, k, v, q_seg, k_seg, scale=0.01)
+    assert want.dq.abs().max() > 0 or n_k == 1
+
+
+@pytest.mark.parametrize("scale", [2.0**-24, 2.0**-12, 4.0])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_cross_scales(scale, dtype):
+    # scores of a few units in each case
+    size = (1.0 / scale / 30) ** 0.5 if scale < 1 else 0.2
+    q, k, v, q_seg, k_seg = attention_inputs(190, lengths_case("few rows on many"), 2, 1, 64, dtype, scale=min(size, 100.0))
+    k *= min(size, 100.0)
+    check_cross(q, k, v, q_seg, k_seg, scale=scale)
+
+
+def test_levels_of_a_hierarchy_together():
+    """A step of an attention network on two rooms: rows and levels of the
+    batched hierarchy, queries and keys turned by the points' coordinates,
+    attention along the radius rows, then of that level's points to the
+    coarser one; forward and backward, eager and captured."""
+    from gsa_b200 import Rotary, cross_attention, cross_attention_grad, hierarchy as hz, neighbor_attention, neighbor_attention_grad, scenes
+
+    sizes, radii, B, H, D = (3000, 750, 187, 46, 11), (0.2, 0.3, 0.5, 0.9), 2, 4, 32
+    X = scenes.room_batch([301, 302], n=sizes[0])
+    batch = hz.Batch(sizes, radii)
+    rows = batch.run(X)["ball1"]
+    near, across = batch.pairs(B, 1, 1), batch.pairs(B, 1, 2)
+    place = X[:, : sizes[1]].reshape(-1, 3)
+    coarse = X[:, : sizes[2]].reshape(-1, 3)
+    turn = Rotary(30, axes=3, unit=0.05)
+    n, m = B * sizes[1], B * sizes[2]
+    q, k, v = (normal(200 + i, n, H, D, dtype=BF16) for i in range(3))
+    k2, v2 = normal(203, m, 2, D, dtype=BF16), normal(204, m, 2, D, dtype=BF16)
+    d = normal(205, n, H, D, dtype=BF16)
+
+    def step():
+        a, b = turn(q, place), turn(k, place)
+        x, lse = neighbor_attention(a, b, v, rows, near, return_lse=True)
+        c, e = turn(x, place), turn(k2, coarse)
+        y, lse2 = cross_attention(c, e, v2, across, return_lse=True)
+        dc, de, dv2 = cross_attention_grad(d, c, e, v2, y, lse2, across)
+        dx = turn.grad(dc, place)
+        da, db, dv = neighbor_attention_grad(dx, a, b, v, rows, x, lse, near)
+        return (x, lse, y, lse2, dx, dv2, dv, turn.grad(da, place), turn.grad(db, place), turn.grad(de, coarse), a, b, c, e, da, db)
+
+    got = step()
+    x, lse, y, lse2, dx, dv2, dv = got[:7]
+    a, b, c, e, da, db = got[10:]
+    near_seg, across_seg = fo.seg_of([sizes[1]] * B), fo.seg_of([sizes[2]] * B)
+    want = fo.Attention(a, b, v, near_seg, near_seg, ids=rows, dout=dx)
+    for name, t in (("out", x), ("lse", lse), ("dq", da), ("dk", db), ("dv", dv)):
+        want.close(name, t)
+    want = fo.Attention(c, e, v2, near_seg, across_seg, dout=d)
+    for name, t in (("out", y), ("lse", lse2), ("dv", dv2)):
+        want.close(name, t)
+    # the same through autograd
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, k2, v2)]
+    f = neighbor_attention(turn(leaves[0], place), turn(leaves[1], place), leaves[2], rows, near)
+    cross_attention(turn(f, place), turn(leaves[3], coarse), leaves[4], across).backward(d)
+    for leaf, t in zip(leaves, (got[7], got[8], dv, got[9], dv2)):
+        assert torch.equal(leaf.grad, t)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for t in (q, v):
+        t.mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, r) for p, r in zip(captured, step()))
+    near.check()
+    across.check()
+
+
 def test_attention_refuses():
     from gsa_b200 import ScenePairs, attention as at
 
@@ -512,6 +610,13 @@ def test_attention_refuses():
         args.update(change)
         with pytest.raises(ValueError):
             at.cross_attention(**args)
+    q.requires_grad_()
+    for call in (lambda: at.cross_attention(q, k, v, pairs, out=out), lambda: at.neighbor_attention(q, k, v, ids, pairs, out=out)):
+        with pytest.raises(ValueError):
+            call()
+    q.requires_grad_(False)
+    with pytest.raises(ValueError):
+        at.cross_attention(normal(1, 9, 65, 16, dtype=BF16), normal(1, 9, 1, 16, dtype=BF16), normal(2, 9, 1, 16, dtype=BF16), pairs)
     for change in bad[1:] + [dict(rows=ids[:8]), dict(rows=ids.long()), dict(rows=ids[:, :0]), dict(rows=ids.cpu()),
                              dict(rows=torch.zeros(9, 33, dtype=torch.int32, device="cuda")), dict(rows=ids.T)]:
         if "q" in change and change["q"].dtype == FP16:
