@@ -22,6 +22,7 @@ from ._library import current_stream
 MAX_DIM = 128
 MAX_WIDTH = 32
 MAX_GROUP = 64  # query heads per head of keys, cross attention
+MAX_SCENES = 65535  # of a cross-attention call
 _INT_MAX = (1 << 31) - 1
 
 
@@ -86,6 +87,8 @@ class _Call:
             raise ValueError("the query heads must be a multiple of the keys' heads")
         if types is _HALF and heads // kv_heads > MAX_GROUP:
             raise ValueError("at most 64 query heads share a head of keys")
+        if types is _HALF and (pairs.scenes > MAX_SCENES or kv_heads > MAX_SCENES):
+            raise ValueError("at most 65535 scenes, and heads of keys, in a call")
         if n_q != pairs.n_q or n_k != pairs.n_k:
             raise ValueError("query and key rows must be those of the pairs' offsets")
         if scale is None:

@@ -23,10 +23,11 @@
 // tensor memory, at most 97 KB of shared memory each).  Below that lie the
 // exponentials (16 a clock on an SM; a quarter are polynomials in the
 // multiply-add units) up to a head of 128, where the products take as long.
-// 8 x 24,000 queries on 6,000 keys, 4 heads of 128: 2.46 ms, 960 TFLOP/s;
-// 8 x 6,000 on 1,500, 8 heads of 64: 250 us, 590 TFLOP/s.  Tiles of 64 keys
-// with four blocks on an SM took 253 to 274 us and 2.7 to 2.8 ms, two threads
-// per row 268 us and 2.68 ms.
+// 8 x 24,000 queries on 6,000 keys, 4 heads of 128: 2.30 to 2.50 ms (the clock
+// falls with the power limit), 945 to 1,020 TFLOP/s; 8 x 6,000 on 1,500, 8
+// heads of 64: 243 us, 607 TFLOP/s.  Tiles of 64 keys with four blocks on an SM
+// took 253 to 274 us and 2.7 to 2.8 ms, two threads per row 268 us and 2.68 ms;
+// no polynomials, or a third, 2 to 3 % more.
 //
 // Where there are too few row tiles to fill the GPU, the keys are split among
 // blocks and the parts joined by their lse.
@@ -54,7 +55,7 @@ struct Shape {
 };
 
 struct Maps {
-  CUtensorMap k, v;
+  CUtensorMap q, k, v;
 };
 
 enum Bar {
@@ -67,7 +68,8 @@ enum Bar {
   kScoresRead = 11,  // S is in registers (a count per warp of rows)
   kWeights = 12,    // P is there (a count per warp of rows)
   kOutput = 13,     // O += P V is complete
-  kBars = 14
+  kQueries = 14,    // Q is there
+  kBars = 15
 };
 
 // The largest of three, NaN if one is.
@@ -86,13 +88,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   __shared__ uint64_t bars[kBars];
   __shared__ uint32_t tmem_at;
 
-  unsigned unit = blockIdx.x;
-  const int r0 = unit % a.tiles * kRows;
-  unit /= a.tiles;
-  const int split = unit % a.splits;
-  unit /= a.splits;
-  const int hk = unit % a.kv_heads;
-  const int scene = unit / a.kv_heads;
+  const int split = a.splits > 1 ? blockIdx.x / a.tiles : 0;
+  const int hk = blockIdx.y, scene = blockIdx.z;
+  const int each = kRows / a.group * a.group;  // whole query rows
+  const int r0 = (blockIdx.x - split * a.tiles) * each;
   const int q0 = __ldg(a.q_seg + scene), k0 = __ldg(a.k_seg + scene);
   const int n = (__ldg(a.q_seg + scene + 1) - q0) * a.group;  // packed rows
   const int nk = __ldg(a.k_seg + scene + 1) - k0;
@@ -167,17 +166,16 @@ __global__ void __launch_bounds__(kThreads, 2)
         tc::barriers_ready();
       }
       __syncwarp();
-      // the first tiles come while the block gets ready
+      // the first tiles come while the block gets ready.  Rows of Q behind the
+      // scene's last hold whatever follows, which no other row sees.
+      if (tc::elect()) {
+        tc::barrier_expect(bar(kQueries), panels * each * 128);
+        for (int p = 0; p < panels; ++p)
+          tc::copy_box(q_tile + p * kRows * 128, &maps.q, bar(kQueries), p * 64,
+                       hk * a.group, q0 + r0 / a.group);
+      }
+      __syncwarp();
       for (int t = 0; t < S::kStages && t < nt; ++t) issue(t);
-    } else {
-      load_packed<T, kRows>(
-          chunks_of(a.dim, tid, kRows), q_tile,
-          static_cast<const T*>(a.q) + q0 * a.q_row +
-              (long long)hk * a.group * a.q_head,
-          a.q_row, a.q_head, a.group, r0, n);
-      tc::copy_commit();
-      tc::copy_wait<0>();
-      tc::fence_shared();
     }
     tc::fence_before();
     __syncthreads();
@@ -204,6 +202,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
     };
     if (nt > 0) {
+      wait(kQueries, 0);
       wait(kKeysFull, 0);
       scores(0);
     }
@@ -235,8 +234,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else {
     const int r = r0 + tid;
-    const bool live = r < n;
-    const bool busy = r0 + warp * 32 < n;  // the warp holds rows
+    const int rows = min(each, n - r0);
+    const bool live = tid < rows;
+    const bool busy = warp * 32 < rows;  // the warp holds rows
     const uint32_t mine = tmem + ((uint32_t)warp << 21);  // the warp's rows
     float m = -kInf, l = 0.f;
     bool seen = false;  // an open key
@@ -379,22 +379,64 @@ __global__ void __launch_bounds__(kThreads, 2)
         else if (a.lse)
           a.lse[at] = lse2 * kLn2;
       }
-      for (int i = 0; i < a.dim; i += 8) {
-        uint32_t x[8];
-        float f[8];
-        __syncwarp();
-        if (seen) {
-          tc::load8(mine + S::kO + i, x);
-          tc::wait_load();
-        }
+      if (a.splits == 1) {
+        // Through Q's place (its products are complete), so that whole rows
+        // are written at a time: chunk c of a row by a lane each.
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          f[e] = none ? 0.f : __uint_as_float(x[e]) * inv;
-        if (!live) continue;
-        if (a.splits == 1) {
-          *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * a.o_row +
-                                    h * a.o_head + i) = Vec<T>::pack(f);
-        } else {
+        for (int i = 0; i < kDim; i += 32) {
+          uint32_t x[32];
+          if (i >= a.dim) break;
+          __syncwarp();
+          if (seen) {
+            tc::load32(mine + S::kO + i, x);
+            tc::wait_load();
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              f[e] = none ? 0.f : __uint_as_float(x[c + e]) * inv;
+            const uint4 u = Vec<T>::pack(f);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             q_tile + tc::tile_offset(kRows, tid, (i + c) / 8)),
+                         "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
+                         : "memory");
+          }
+        }
+        __syncwarp();
+        constexpr int kChunks = kDim / 8, kAtOnce = 32 / kChunks;
+        const int chunk = lane % kChunks;
+        if (chunk * 8 < a.dim) {
+#pragma unroll 4
+          for (int i = lane / kChunks; i < 32; i += kAtOnce) {
+            const int w = warp * 32 + i;
+            if (w >= rows) break;
+            uint4 u;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                         : "r"(q_tile + tc::tile_offset(kRows, w, chunk))
+                         : "memory");
+            const int p = (r0 + w) / a.group;
+            const int head = hk * a.group + (r0 + w - p * a.group);
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.o) +
+                                      (q0 + p) * a.o_row + head * a.o_head +
+                                      chunk * 8) = u;
+          }
+        }
+      } else {
+        for (int i = 0; i < a.dim; i += 8) {
+          uint32_t x[8];
+          float f[8];
+          __syncwarp();
+          if (seen) {
+            tc::load8(mine + S::kO + i, x);
+            tc::wait_load();
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            f[e] = none ? 0.f : __uint_as_float(x[e]) * inv;
+          if (!live) continue;
           float4* o = reinterpret_cast<float4*>(a.part + at * a.dim + i);
           o[0] = make_float4(f[0], f[1], f[2], f[3]);
           o[1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -484,15 +526,15 @@ __global__ void __launch_bounds__(128)
 }
 
 template <typename T, int kDim>
-cudaError_t launch(const CrossArgs& a, const Maps& maps, long long units,
-                   cudaStream_t s) {
+cudaError_t launch(const CrossArgs& a, const Maps& maps, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(
       cross_forward_kernel<T, kDim>,
       cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<kDim>::kSmem);
   if (e) return e;
   count_launches(1);
+  const dim3 grid(a.tiles * a.splits, a.kv_heads, a.scenes);
   cross_forward_kernel<T, kDim>
-      <<<(unsigned)units, kThreads, Shape<kDim>::kSmem, s>>>(a, maps);
+      <<<grid, kThreads, Shape<kDim>::kSmem, s>>>(a, maps);
   if (a.splits > 1) {
     count_launches(1);
     cross_join_kernel<T>
@@ -537,6 +579,7 @@ bool cross_sizes(const attention_args* a) {
   return attention_sizes(a) && a->type != kF32 &&
          a->heads / a->kv_heads <= 64 && a->max_q >= 0 &&
          a->max_q <= a->n_q && a->max_k >= 0 && a->max_k <= a->n_k &&
+         a->scenes <= 65535 && a->kv_heads <= 65535 &&  // a grid's limits
          a->max_q * (a->heads / a->kv_heads) < kMaxInt - 2 * kRows &&
          a->max_k < kMaxInt - 2 * kRows;
 }
@@ -631,7 +674,8 @@ struct ForwardPlan {
 
 ForwardPlan forward_plan(const attention_args* a) {
   ForwardPlan p;
-  p.tiles = ceil_div(a->max_q * (a->heads / a->kv_heads), kRows);
+  const long long group = a->heads / a->kv_heads;
+  p.tiles = ceil_div(a->max_q * group, kRows / group * group);
   const long long blocks = p.tiles * a->scenes * a->kv_heads;
   p.splits = split_count(blocks, ceil_div(a->max_k, kKeys),
                          2 * multiprocessors());
@@ -672,7 +716,10 @@ GSA_API int cross_attention(const attention_args* in) {
   if (p.splits > 1) a.part_lse = a.part + p.splits * a.n_q * a.heads * a.dim;
   Maps maps = {};
   if (in->n_k) {
-    cudaError_t e = row_map(&maps.k, in->type, in->k, a.dim, a.kv_heads, a.n_k,
+    cudaError_t e = row_map(&maps.q, in->type, in->q, a.dim, a.heads, a.n_q,
+                            a.group, kRows / a.group);
+    if (!e)
+      e = row_map(&maps.k, in->type, in->k, a.dim, a.kv_heads, a.n_k,
                             1, kKeys);
     if (!e)
       e = row_map(&maps.v, in->type, in->v, a.dim, a.kv_heads, a.n_k, 1, kKeys);
@@ -680,8 +727,8 @@ GSA_API int cross_attention(const attention_args* in) {
   }
   cudaStream_t s = (cudaStream_t)in->stream;
   if (in->type == kF16)
-    return a.dim <= 64 ? launch<__half, 64>(a, maps, p.blocks, s)
-                       : launch<__half, 128>(a, maps, p.blocks, s);
-  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, maps, p.blocks, s)
-                     : launch<__nv_bfloat16, 128>(a, maps, p.blocks, s);
+    return a.dim <= 64 ? launch<__half, 64>(a, maps, s)
+                       : launch<__half, 128>(a, maps, s);
+  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, maps, s)
+                     : launch<__nv_bfloat16, 128>(a, maps, s);
 }

@@ -62,7 +62,7 @@ BAD_SIZES = [dict(type=3), dict(type=-1), dict(scenes=0), dict(n_q=-1), dict(n_k
 
 @pytest.mark.parametrize("bad", BAD_SIZES + [
     dict(type=0), dict(max_q=5), dict(max_q=-1), dict(max_k=9), dict(scale=0.0), dict(scale=-1.0),
-    dict(scale=2.0**-25), dict(scale=2.0**25), dict(heads=65, q=(1 << 20, 65 * 16, 16), out=(1 << 20, 65 * 16, 16)),
+    dict(scale=2.0**-25), dict(scale=2.0**25), dict(scenes=65536), dict(heads=65, q=(1 << 20, 65 * 16, 16), out=(1 << 20, 65 * 16, 16)),
     dict(scale=math.inf), dict(scale=math.nan), dict(q=(0, 32, 16)), dict(q=((1 << 20) + 2, 32, 16)),
     dict(q=(1 << 20, 33, 16)), dict(k=(1 << 20, 16, 4)), dict(v=(0, 16, 16)), dict(out=((1 << 20) + 8, 32, 16)),
     dict(q_seg=0), dict(k_seg=0), dict(error=0)], ids=str)
