@@ -105,6 +105,8 @@ class Rotary:
         else:
             to = ft.rows_of(out, "out", shape, dtype, device)
             ft.check_written(out, "out")
+            if to[0] == place[0] and to != place:
+                raise ValueError("out may be the rows themselves, not another view of them")
         steps = positions.stride()
         args = ft.pack_rotary(
             ft.TYPES[dtype], rows, heads, dim, *place, *to, positions.data_ptr(), kind, steps[0], steps[1] if axes else 0,

@@ -113,7 +113,7 @@ def test_rotary_refuses():
                 (x, place.double()), (x, place.cpu()), (x, place[:, None].expand(6, 2)), (x[:, :0], place)]:
         with pytest.raises(ValueError):
             r(*bad)
-    for out in (x[:5], x.half(), x.cpu(), x[:, :1].expand(6, 2, 32)):
+    for out in (x[:5], x.half(), x.cpu(), x[:, :1].expand(6, 2, 32), x.view(2, 6, 32).transpose(0, 1)):
         with pytest.raises(ValueError):
             r(x, place, out=out)
 
