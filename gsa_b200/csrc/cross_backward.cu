@@ -123,8 +123,8 @@ __device__ __forceinline__ void product_more(uint32_t d, uint32_t a,
           tc::instruction<T>(kN, false), true);
 }
 
-// kOneTile: no scene has more walked rows than a tile (queries' pass).
-template <typename T, int kDim, bool kKeysPass, bool kOneTile>
+// kFew (queries' pass): scenes may have their keys in one tile.
+template <typename T, int kDim, bool kKeysPass, bool kFew>
 __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
                                   Shape<kDim, kKeysPass>::kBlocks)
     cross_backward_kernel(const __grid_constant__ CrossArgs a,
@@ -153,6 +153,9 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
   int begin, end;
   share((walked + each - 1) / each, a.splits, split, &begin, &end);
   const int nt = end - begin;
+  // All keys are in one tile: delta is the sum of P * dP, without the rounding
+  // of `out`, which would be most of dS's error where keys are few.
+  const bool one_tile = kFew && nk <= W;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         for (int i = 0; i < kEach; ++i) {
           const int at = ((tid >> 7) + i * S::kShare) * 8;
           u[i] = v[i] = make_uint4(0, 0, 0, 0);
-          if (!kOneTile && at < a.dim) {
+          if (!one_tile && at < a.dim) {
             u[i] = *reinterpret_cast<const uint4*>(o + at);
             v[i] = *reinterpret_cast<const uint4*>(d + at);
           }
@@ -426,7 +429,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
     if constexpr (kKeysPass) {
       open = live && (!mask || __ldg(mask + r));
     } else if (nt > 0) {
-      if constexpr (!kOneTile) {
+      if (!one_tile) {
 #pragma unroll
         for (int i = 0; i < S::kShare; ++i)
           delta += part_delta[i][group * 32 + lane];
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         // a row without keys gets P = 0
         const float x = __ldg(a.lse + row * a.heads + h);
         if (x != -kInf) lse2 = fmaf(x, -kLog2e, (float)p_bits<T>());
-        if (!kOneTile && part == 0) put_values(-delta);
+        if (!one_tile && part == 0) put_values(-delta);
       }
       delta *= -ds_factor;
     }
@@ -482,9 +485,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
           const int first = (begin + t) * W;
           some = mask || first + W > nk;
           if (some) key_words<W>(words, mask, first, nk);
-          if constexpr (kOneTile) {
-            // All keys are here: delta is the sum of P * dP, without the
-            // rounding of `out` (of few keys its largest error).
+          if (one_tile) {
             float sum = 0.f;
             const uint32_t word = some ? my_word(words) : 0xffffffffu;
 #pragma unroll
@@ -675,7 +676,7 @@ Plan backward_plan(const attention_args* a) {
   return p;
 }
 
-template <typename T, int kDim, bool kKeysPass, bool kOneTile>
+template <typename T, int kDim, bool kKeysPass, bool kFew>
 cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
                         cudaStream_t s) {
   using S = Shape<kDim, kKeysPass>;
@@ -699,12 +700,12 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
                   S::kWalk);
   }
   if (!e)
-    e = cudaFuncSetAttribute(cross_backward_kernel<T, kDim, kKeysPass, kOneTile>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           S::kSmem);
+    e = cudaFuncSetAttribute(cross_backward_kernel<T, kDim, kKeysPass, kFew>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             S::kSmem);
   if (e) return e;
   count_launches(1);
-  cross_backward_kernel<T, kDim, kKeysPass, kOneTile>
+  cross_backward_kernel<T, kDim, kKeysPass, kFew>
       <<<(unsigned)grid, S::kThreads, S::kSmem, s>>>(a, maps);
   if (a.splits > 1) {
     const long long n =
@@ -725,16 +726,20 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
 }
 
 // The queries' pass first: it leaves its rows' lse and delta to the keys'.
+// Scenes of one tile of keys beside others of many take delta from `out` like
+// those: looking for them costs the pass registers (8 scenes of 6000 rows and
+// 1500 keys, both passes: 945 us, without 920), and a batch whose largest has
+// 16 tiles and more has little of its gradients from them.
 template <typename T>
 cudaError_t launch(const CrossArgs& a, const attention_args* in, const Plan& p,
                    cudaStream_t s) {
   cudaError_t e;
   if (a.dim <= 64)
-    e = in->max_k <= Shape<64, false>::kWalk
+    e = in->max_k <= 16 * Shape<64, false>::kWalk
             ? launch_pass<T, 64, false, true>(a, in, p, s)
             : launch_pass<T, 64, false, false>(a, in, p, s);
   else
-    e = in->max_k <= Shape<128, false>::kWalk
+    e = in->max_k <= 16 * Shape<128, false>::kWalk
             ? launch_pass<T, 128, false, true>(a, in, p, s)
             : launch_pass<T, 128, false, false>(a, in, p, s);
   if (e) return e;

@@ -522,6 +522,26 @@ def test_cross_gradients_of_few_keys(n_k, dim, dtype):
     assert want.dq.abs().max() > 0 or n_k == 1
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16)])
+def test_cross_gradients_of_few_keys_beside_many(dim, dtype):
+    # a scene of one tile of keys keeps its own path beside one of several, so
+    # its gradients are the bits that it has alone
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(185, ([130, 40], [5, 300]), 2, 1, dim, dtype)
+    check_cross(q, k, v, q_seg, k_seg)
+    d = normal(186, *q.shape, dtype=dtype)
+
+    def gradients(d, q, k, v, pairs):
+        out, lse = cross_attention(q, k, v, pairs, return_lse=True)
+        return cross_attention_grad(d, q, k, v, out, lse, pairs)
+
+    both = gradients(d, q, k, v, ScenePairs(q_seg, k_seg))
+    alone = gradients(d[:130], q[:130], k[:5], v[:5], ScenePairs([0, 130], [0, 5]))
+    for got, want in zip(both, alone):
+        assert torch.equal(got[: len(want)], want)
+
+
 @pytest.mark.parametrize("scale", [2.0**-24, 2.0**-12, 4.0])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_cross_scales(scale, dtype):
