@@ -66,7 +66,7 @@ def vector_rows_of(t, what, shape, dtype, device):
 
 
 def check_written(t, what):
-    """A tensor to write to: no two of its elements share memory."""
+    """A tensor about to be written: no two of its elements share memory."""
     (a, n), (b, m) = sorted(zip(t.stride()[:2], t.shape[:2]))
     least = t.shape[2]
     for stride, size in ((a, n), (b, m)):
@@ -74,3 +74,5 @@ def check_written(t, what):
             if stride < least:
                 raise ValueError(f"{what}: elements overlap")
             least = stride * (size - 1) + least
+    # a backward pass that saved the tensor learns that it was written
+    torch.autograd.graph.increment_version(t)

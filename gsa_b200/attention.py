@@ -45,7 +45,7 @@ class ScenePairs:
         self.n_q, self.n_k = q_seg[-1], k_seg[-1]
         self.max_q = max(b - a for a, b in zip(q_seg, q_seg[1:]))
         self.max_k = max(b - a for a, b in zip(k_seg, k_seg[1:]))
-        self.device = current_stream()[0]
+        self.device, self.stream = current_stream()
         # both offset lists, and the flag of the kernels' bounded waits
         self._ints = torch.tensor(q_seg + k_seg + [0], dtype=torch.int32).to(f"cuda:{self.device}")
         self._q_at = self._ints.data_ptr()
@@ -95,6 +95,9 @@ class _Call:
             scale = dim ** -0.5
         if not 2.0**-24 <= scale <= 2.0**24:
             raise ValueError("scale must be positive, from 2^-24 to 2^24")
+        if self.stream != pairs.stream:
+            # the offsets outlive the pairs until this stream is done with them
+            pairs._ints.record_stream(torch.cuda.current_stream())
         self.what, self.dtype, self.pairs, self.on = what, q.dtype, pairs, q.device
         self.q_shape, self.k_shape = (n_q, heads, dim), (n_k, kv_heads, dim)
         self.sizes = (ft.TYPES[q.dtype], pairs.scenes, n_q, n_k, pairs.max_q, pairs.max_k, heads, kv_heads, dim, scale)
@@ -162,10 +165,10 @@ class _Call:
             _, heads, dim = self.q_shape
             place = (out.data_ptr(), heads * dim, dim)
         else:
-            place = self.rows_of(out, "out", self.q_shape)
-            ft.check_written(out, "out")
+            place = ft.vector_rows_of(out, "out", self.q_shape, self.dtype, self.device)
             if place[0] and place[0] in [t.data_ptr() for t in inputs]:
                 raise ValueError("out must not overlap the inputs")
+            ft.check_written(out, "out")
         if not return_lse:
             self.run(entry, workspace, place, (0, 0, 0), 0, (0, 0, 0))
             return out
@@ -245,8 +248,10 @@ def neighbor_attention(q, k, v, rows, pairs, padded=True, scale=None, out=None, 
     scene's keys (a negative one) is absent.  ``padded``: an entry that
     repeats the row's first is absent too, as behind the hits of a radius
     row; else repeats count each time.  (A radius row without hits is all
-    zeros and reads key 0, like any such row of a radius query.)  ``q``,
-    ``k``, ``v`` and the rest as for ``cross_attention``, FP32 too."""
+    zeros and reads key 0, like any such row of a radius query.)  The rows keep
+    their values until the gradient is taken: a query that writes the same
+    buffer again is not noticed.  ``q``, ``k``, ``v`` and the rest as for
+    ``cross_attention``, FP32 too."""
     if _wants_grad(out, q, k, v):
         out, lse = _Neighbor.apply(q, k, v, rows, pairs, padded, scale)
         return (out, lse) if return_lse else out

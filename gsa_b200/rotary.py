@@ -19,6 +19,7 @@ from ._library import current_stream
 
 MAX_PAIRS = 128  # per axis
 MAX_DIM = 4096
+MAX_AMPLITUDE = torch.finfo(torch.float32).max
 
 
 def frequencies(pairs, base=10000.0, scaling=None, factor=1.0, length=None, low=1.0, high=32.0):
@@ -70,8 +71,8 @@ class Rotary:
             raise ValueError("scaling 'ramp' needs the length trained on")
         if amplitude is None:
             amplitude = 0.1 * math.log(factor) + 1.0 if scaling == "ramp" else 1.0
-        if not math.isfinite(amplitude):
-            raise ValueError("amplitude must be finite")
+        if not abs(amplitude) <= MAX_AMPLITUDE:
+            raise ValueError("amplitude must be finite in FP32")
         self.part, self.axes, self.layout, self.amplitude = part, axes, layout, amplitude
         self.pairs = part // (2 * axes)
         self._interleaved = layout == "interleaved"
@@ -104,9 +105,9 @@ class Rotary:
             to = (out.data_ptr(), heads * dim, dim)
         else:
             to = ft.rows_of(out, "out", shape, dtype, device)
-            ft.check_written(out, "out")
-            if to[0] == place[0] and to != place:
+            if to[0] == place[0] and to != place and out.numel():
                 raise ValueError("out may be the rows themselves, not another view of them")
+            ft.check_written(out, "out")
         steps = positions.stride()
         args = ft.pack_rotary(
             ft.TYPES[dtype], rows, heads, dim, *place, *to, positions.data_ptr(), kind, steps[0], steps[1] if axes else 0,

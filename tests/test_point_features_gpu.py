@@ -118,6 +118,45 @@ def test_rotary_refuses():
             r(x, place, out=out)
 
 
+def test_writes_are_known_to_autograd():
+    from gsa_b200 import Rotary, ScenePairs, cross_attention
+
+    q, k, v, q_seg, k_seg = attention_inputs(195, ([40], [60]), 2, 2, 32, BF16)
+    pairs, r = ScenePairs(q_seg, k_seg), Rotary(32)
+    for write in (lambda t: r(q, torch.arange(40).cuda(), out=t), lambda t: cross_attention(q, k, v, pairs, out=t)):
+        buffer = torch.ones_like(q)
+        leaf = normal(196, *q.shape, dtype=BF16).requires_grad_()
+        product = leaf * buffer
+        write(buffer)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+    with torch.inference_mode():
+        out = torch.empty_like(q)
+        assert cross_attention(q, k, v, pairs, out=out) is out
+    empty = q[:0]
+    assert r(empty, torch.arange(0).cuda(), out=torch.empty((0, 2, 64), dtype=BF16, device="cuda")[..., :32]).shape == empty.shape
+    with pytest.raises(ValueError):
+        Rotary(32, amplitude=1e39)
+
+
+def test_pairs_end_before_another_stream_has_read_them():
+    from gsa_b200 import ScenePairs, cross_attention
+
+    q, k, v, q_seg, k_seg = attention_inputs(197, ([500, 700], [900, 400]), 2, 2, 64, BF16)
+    pairs = ScenePairs(q_seg, k_seg)
+    want = cross_attention(q, k, v, pairs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(50):  # work that the call below waits for
+            (q.float() @ q.float().mT)
+        got = cross_attention(q, k, v, pairs)
+    del pairs
+    later = [torch.zeros(7, dtype=torch.int32, device="cuda") for _ in range(64)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(later) == 64
+
+
 # ---------------------------------------------------------------------------
 # attention
 
