@@ -21,7 +21,16 @@
 // multiplied and added in 32 bits.  So nothing is done twice: a block first
 // lists the entries that count of its rows (once for all heads) in shared
 // memory; a head is a group of lanes with a 16-byte vector each, with several
-// entries' loads in flight, multiplying pairs at a time.
+// entries' loads in flight, multiplying pairs at a time.  Every lane of a group
+// takes the whole sum of a product: sharing the entries' sums and exponentials
+// out among the lanes saves instructions but lengthens the chain from load to
+// result (397 us for 388 forward, 488 for 464 forward and back).
+//
+// 192,000 rows of 32 entries, 8 heads of 32 in bf16: 388 us, 1.08 TB/s of
+// tensors in device memory (418 MB) and 12 TB/s of gathered heads through L1 and
+// L2.  48,000 rows, 4 heads of 32 in FP32, forward and back: 464 us, of them
+// about 105 forward, 95 for the order of the entries, 110 for dq and 185 for dk
+// and dv.
 #include "features.cuh"
 #include "tensor_core.cuh"
 
@@ -40,13 +49,19 @@ struct NeighborArgs {
   long long n_q, n_k;
   long long q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, d_row,
       d_head;
+  // rows' strides in bytes, of what is gathered: a 32-bit one times a row is
+  // one instruction
+  uint32_t q_step, k_step, v_step, d_step;
   int scenes, heads, kv_heads, group, dim, width, padded;
   float scale, scale_log2e;
 };
 
 constexpr int kBlock = 128;
-// Entries of a group whose loads are in flight: with 8 (or 2) the forward pass
-// of 192,000 rows takes 654 (549) us instead of 514.
+// Blocks of an SM (64 registers a thread): the forward pass of 192,000 rows
+// takes 388 us, with 7 (72 registers) 431, with 9 (spills) 476.
+constexpr int kResident = 8;
+// Entries of a group whose loads are in flight (an earlier form of the forward
+// pass: 514 us with 4, 654 with 8, 549 with 2).
 constexpr int kAhead = 4;
 constexpr int kListStride = 36;    // of a row's list, clear of bank conflicts
 
@@ -128,6 +143,13 @@ __device__ __forceinline__ float dot(const uint4& a, const uint4& b) {
   }
 }
 
+// A row's vector; rows from 0 on.
+__device__ __forceinline__ uint4 gather(const void* base, int row,
+                                        uint32_t step) {
+  return __ldg(reinterpret_cast<const uint4*>(
+      static_cast<const char*>(base) + (uint64_t)(uint32_t)row * step));
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 vector_at(const void* base, long long element) {
   return __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) +
@@ -193,13 +215,22 @@ struct Group {
     keys = lists.keys[row - row0];
     n = live ? lists.count[row - row0] : 0;
     const int hk = h / a.group;
-    k = static_cast<const T*>(a.k) + hk * a.k_head + j * V;
-    v = static_cast<const T*>(a.v) + hk * a.v_head + j * V;
+    // a lane without a vector reads the first, and takes no part (`sum`)
+    const int at = mine ? j * V : 0;
+    k = static_cast<const T*>(a.k) + hk * a.k_head + at;
+    v = static_cast<const T*>(a.v) + hk * a.v_head + at;
   }
 
-  // The vectors of kAhead entries from j0 on.
+  // The group's sum of its lanes' parts.
+  __device__ __forceinline__ float sum(float part) const {
+    return group_sum<L>(mine ? part : 0.f);
+  }
+
+  // The vectors of kAhead entries from j0 on; behind the last entry they stay
+  // as they are, and what comes of them is not used.
   __device__ __forceinline__ void load(const NeighborArgs& a, int j0,
                                        uint4* ku, uint4* vu) const {
+    if (j0 >= n) return;
     int at[kAhead];
 #pragma unroll
     for (int t = 0; t < kAhead; t += 4)
@@ -207,17 +238,14 @@ struct Group {
           *reinterpret_cast<const int4*>(keys + j0 + t);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      ku[t] = vu[t] = make_uint4(0, 0, 0, 0);
-      if (mine && j0 < n) {
-        ku[t] = __ldg(reinterpret_cast<const uint4*>(k + at[t] * a.k_row));
-        vu[t] = __ldg(reinterpret_cast<const uint4*>(v + at[t] * a.v_row));
-      }
+      ku[t] = gather(k, at[t], a.k_step);
+      vu[t] = gather(v, at[t], a.v_step);
     }
   }
 };
 
 template <typename T, int L>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, kResident)
     neighbor_forward_kernel(const __grid_constant__ NeighborArgs a) {
   __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
   const Group<T, L> g(a, lists);
@@ -227,13 +255,13 @@ __global__ void __launch_bounds__(kBlock)
   if (g.mine)
     q = vector_at<T>(a.q, g.row * a.q_row + g.h * a.q_head + g.j * Vec<T>::V);
   float m = -kInf, l = 0.f;
+  uint4 ku[kAhead] = {}, vu[kAhead] = {};
   for (int j0 = 0; __any_sync(kFull, j0 < g.n); j0 += kAhead) {
-    uint4 ku[kAhead], vu[kAhead];
     g.load(a, j0, ku, vu);
     float s[kAhead], top = m;
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      s[t] = group_sum<L>(dot<T>(ku[t], q)) * a.scale_log2e;
+      s[t] = g.sum(dot<T>(ku[t], q)) * a.scale_log2e;
       if (j0 + t >= g.n) s[t] = -kInf;
       top = fmaxf(top, s[t]);
     }
@@ -262,7 +290,7 @@ __global__ void __launch_bounds__(kBlock)
 
 // dq, and delta for the keys' pass.
 template <typename T, int L>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, kResident)
     neighbor_dq_kernel(const __grid_constant__ NeighborArgs a) {
   __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
   const Group<T, L> g(a, lists);
@@ -280,13 +308,13 @@ __global__ void __launch_bounds__(kBlock)
   const float delta = group_sum<L>(part);
   if (g.live && g.j == 0) a.delta[g.unit] = delta;
   const float lse2 = g.live ? __ldg(a.lse + g.unit) * kLog2e : 0.f;
+  uint4 ku[kAhead] = {}, vu[kAhead] = {};
   for (int j0 = 0; __any_sync(kFull, j0 < g.n); j0 += kAhead) {
-    uint4 ku[kAhead], vu[kAhead];
     g.load(a, j0, ku, vu);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      const float s = group_sum<L>(dot<T>(ku[t], q));
-      const float dp = group_sum<L>(dot<T>(vu[t], d));
+      const float s = g.sum(dot<T>(ku[t], q));
+      const float dp = g.sum(dot<T>(vu[t], d));
       const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2));
       if (j0 + t < g.n) acc.add(p * (dp - delta), Pairs<T>(ku[t]));
     }
@@ -301,12 +329,12 @@ __global__ void __launch_bounds__(kBlock)
 // dk and dv: a warp per (key, head of keys); its 32 / L groups take the key's
 // (entry, query head) pairs in turn and are added up at the end.
 template <typename T, int L>
-__global__ void __launch_bounds__(kBlock, 8)
+__global__ void __launch_bounds__(kBlock, kResident)
     neighbor_dkv_kernel(const __grid_constant__ NeighborArgs a) {
   constexpr int V = Vec<T>::V;
   constexpr int G = 32 / L;
-  // Entries of a group in flight: more warps (64 registers) are worth more
-  // here (4 with 96 registers: 571 us of the training case, so: 503).
+  // Entries of a group in flight: more warps are worth more here (4 with 96
+  // registers: 571 us of 48,000 rows forward and back, so: 503).
   constexpr int kDeep = 2;
   const long long unit =
       ((long long)blockIdx.x * kBlock + threadIdx.x) >> 5;
@@ -315,20 +343,23 @@ __global__ void __launch_bounds__(kBlock, 8)
   const long long key = unit / a.kv_heads;
   const int hk = (int)(unit - key * a.kv_heads);
   const bool mine = j * V < a.dim;
+  const int first = mine ? j * V : 0;  // a lane without a vector: the first
   Pairs<T> dk, dv;
   dk.clear();
   dv.clear();
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (mine) {
-    k = vector_at<T>(a.k, key * a.k_row + hk * a.k_head + j * V);
-    v = vector_at<T>(a.v, key * a.v_row + hk * a.v_head + j * V);
-  }
+  const uint4 k =
+      vector_at<T>(a.k, key * a.k_row + hk * a.k_head + first);
+  const uint4 v =
+      vector_at<T>(a.v, key * a.v_row + hk * a.v_head + first);
+  uint4 qu[kDeep] = {}, du[kDeep] = {};
   const int from = __ldg(a.starts + key), to = __ldg(a.starts + key + 1);
   for (int e0 = from; e0 < to; e0 += 32) {
     // an entry's row and its values in a lane each
     const int n = min(32, to - e0);
     const int mine_row = lane < n ? __ldg(a.order + e0 + lane) : 0;
     for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
+      const T* q = static_cast<const T*>(a.q) + h * a.q_head + first;
+      const T* d = static_cast<const T*>(a.dout) + h * a.d_head + first;
       float mine_lse = 0.f, mine_delta = 0.f;
       if (lane < n) {
         const long long at = (long long)mine_row * a.heads + h;
@@ -336,24 +367,22 @@ __global__ void __launch_bounds__(kBlock, 8)
         mine_delta = __ldg(a.delta + at);
       }
       for (int t0 = 0; t0 < n; t0 += G * kDeep) {
-        uint4 qu[kDeep], du[kDeep];
         float lse2[kDeep], delta[kDeep];
 #pragma unroll
         for (int t = 0; t < kDeep; ++t) {
           const int e = t0 + t * G + who;
-          const long long row = __shfl_sync(kFull, mine_row, e & 31);
+          const int row = __shfl_sync(kFull, mine_row, e & 31);
           lse2[t] = __shfl_sync(kFull, mine_lse, e & 31);
           delta[t] = __shfl_sync(kFull, mine_delta, e & 31);
-          qu[t] = du[t] = make_uint4(0, 0, 0, 0);
-          if (mine && e < n) {
-            qu[t] = vector_at<T>(a.q, row * a.q_row + h * a.q_head + j * V);
-            du[t] = vector_at<T>(a.dout, row * a.d_row + h * a.d_head + j * V);
+          if (e < n) {
+            qu[t] = gather(q, row, a.q_step);
+            du[t] = gather(d, row, a.d_step);
           }
         }
 #pragma unroll
         for (int t = 0; t < kDeep; ++t) {
-          const float s = group_sum<L>(dot<T>(qu[t], k));
-          const float dp = group_sum<L>(dot<T>(du[t], v));
+          const float s = group_sum<L>(mine ? dot<T>(qu[t], k) : 0.f);
+          const float dp = group_sum<L>(mine ? dot<T>(du[t], v) : 0.f);
           if (t0 + t * G + who >= n) continue;
           const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2[t]));
           dk.add(p * (dp - delta[t]), Pairs<T>(qu[t]));
@@ -617,6 +646,14 @@ cudaError_t run_type(const NeighborArgs& a, int type, bool back,
   return run<__nv_bfloat16>(a, back, s);
 }
 
+// A gathered tensor's stride from row to row, in bytes.
+bool step_of(const feature_rows& t, long long rows, long long type,
+             uint32_t* step) {
+  const long long bytes = rows > 1 ? t.row * (type == kF32 ? 4 : 2) : 0;
+  *step = (uint32_t)bytes;
+  return bytes >= 0 && bytes <= 0xffffffffll;
+}
+
 bool sizes_ok(const attention_args* a) {
   return attention_sizes(a) && a->width >= 1 && a->width <= 32 &&
          a->n_q * a->width < kMaxInt;
@@ -668,6 +705,9 @@ GSA_API int neighbor_attention(const attention_args* in) {
       (!vector_rows(in->k, in->type) || !vector_rows(in->v, in->type)))
     return -2;
   NeighborArgs a = arguments(in);
+  if (!step_of(in->k, in->n_k, in->type, &a.k_step) ||
+      !step_of(in->v, in->n_k, in->type, &a.v_step))
+    return -2;
   a.o = const_cast<void*>(in->out.data);
   a.lse_out = in->lse;
   return run_type(a, (int)in->type, false, (cudaStream_t)in->stream);
@@ -700,6 +740,11 @@ GSA_API int neighbor_attention_grad(const attention_args* in) {
       in->workspace_bytes < neighbor_attention_grad_workspace(in))
     return -2;
   NeighborArgs a = arguments(in);
+  if (!step_of(in->q, n_q, type, &a.q_step) ||
+      !step_of(in->dout, n_q, type, &a.d_step) ||
+      !step_of(in->k, n_k, type, &a.k_step) ||
+      !step_of(in->v, n_k, type, &a.v_step))
+    return -2;
   a.out = in->out.data;
   a.dout = in->dout.data;
   a.d_row = in->dout.row;
