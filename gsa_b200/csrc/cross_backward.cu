@@ -35,7 +35,11 @@
 //
 // What bounds it, for 128 x 128 scores and a head of 64: 1,400 clocks of
 // products in the keys' pass (1,024 in the queries') beside 1,024 of
-// exponentials.
+// exponentials.  A tile takes some 2,580 clocks there: its chain of scores,
+// softmax, weights and products, of which only the next scores run ahead.  8 x
+// 6,000 queries on 1,500 keys, 8 heads of 64 in bf16: about 330 us of the
+// queries' pass and 350 of the keys', 540 TFLOP/s of the five products that
+// count.
 #include "cross.cuh"
 
 namespace gsa {

@@ -32,7 +32,9 @@ extern "C" {
 #define POINT_FEATURES_F16 1
 #define POINT_FEATURES_BF16 2
 
-/* A tensor of rows: strides in elements. */
+/* A tensor of rows: strides in elements.  Attention reads and writes 16 bytes
+ * at a time: its tensors start on 16 bytes and their strides are multiples of
+ * 16 bytes. */
 typedef struct {
   const void* data;
   int64_t row, head;
@@ -61,10 +63,14 @@ typedef struct {
   int64_t type, scenes, n_q, n_k;
   int64_t max_q, max_k;     /* longest scene */
   int64_t heads, kv_heads;  /* heads a multiple of kv_heads: head h reads
-                               head h / (heads / kv_heads) of the keys */
+                               head h / (heads / kv_heads) of the keys; cross
+                               attention: at most 64 heads per kv_head, 65535
+                               kv_heads and 65535 scenes */
   int64_t dim;              /* a multiple of 8, at most 128 */
   double scale;             /* 2^-24 to 2^24 */
-  feature_rows q, k, v;
+  feature_rows q, k, v;     /* cross: no strides of 0 or from 2^40 bytes on;
+                               neighbor: row strides of what is gathered (k,
+                               v; backward q and dout too) below 2^32 bytes */
   feature_rows out;         /* written forward, read backward */
   feature_rows dout;
   float* lse;               /* [n_q][heads], natural log; may be null forward */

@@ -78,6 +78,16 @@ def test_cross_gradient_entry_refuses(bad):
     assert ft.lib.cross_attention_grad(cross_args(**bad)) == -2
 
 
+@pytest.mark.parametrize("name", ["k", "v", "q", "dout"])
+@pytest.mark.parametrize("row", [1 << 31, -32])
+def test_neighbor_entry_refuses_rows_too_far_apart(name, row):
+    # a gathered tensor's row stride is 32 bits of bytes
+    bad = cross_args(**{name: (1 << 20, row, 16)})
+    assert ft.lib.neighbor_attention_grad(bad) == -2
+    if name in "kv":
+        assert ft.lib.neighbor_attention(bad) == -2
+
+
 @pytest.mark.parametrize("bad", BAD_SIZES + [
     dict(width=0), dict(width=33), dict(ids=0), dict(q=(1 << 20, 33, 16)), dict(k=(0, 16, 16)),
     dict(v=((1 << 20) + 8, 16, 16)), dict(out=(0, 32, 16)), dict(q_seg=0), dict(k_seg=0), dict(scale=0.0)], ids=str)
