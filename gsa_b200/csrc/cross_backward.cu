@@ -449,6 +449,20 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
       }
       delta *= -ds_factor;
     }
+    // A scene's only open key has P = 1 whatever the scores, and dS = 0 (looked
+    // for where all keys are in a tile).
+    bool lone = false;
+    if constexpr (kKeysPass || kFew) {
+      constexpr int kLook = kKeysPass ? kRows : W;
+      if (nk <= kLook) {
+        uint32_t words[kLook / 32];
+        key_words<kLook>(words, mask, 0, nk);
+        int keys = 0;
+#pragma unroll
+        for (int i = 0; i < kLook / 32; ++i) keys += __popc(words[i]);
+        lone = keys == 1;
+      }
+    }
     __syncwarp();
     const bool all_open = __all_sync(kFull, open);
     const uint64_t scale2 = tc::pair(a.scale_log2e, a.scale_log2e);
@@ -549,6 +563,14 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
               ds[i] &= ((two & 1) ? 0xffffu : 0u) |
                        ((two & 2) ? 0xffff0000u : 0u);
             }
+          }
+        }
+        if (lone) {
+#pragma unroll
+          for (int i = 0; i < kMine / 2; ++i) {  // 0, or NaN of what is one
+            float w[2];
+            Vec<T>::unpack2(ds[i], w);
+            ds[i] = pack2<T>(w[0] - w[0], w[1] - w[1]);
           }
         }
         // P's and dS's places are free once the last products are complete

@@ -288,15 +288,21 @@ __global__ void __launch_bounds__(kBlock, kResident)
     a.lse_out[g.unit] = g.n ? (m + log2f(l)) * kLn2 : -kInf;
 }
 
-// dq, and delta for the keys' pass.
+// dq, and delta for the keys' pass.  Of few entries the rounding of a 16-bit
+// `out` would be most of the error of ds, so that <dout, out> only serves as a
+// start d0 there: with ds0 = p (dp - d0) and c = sum ds0, delta = d0 + c and
+// dq = scale (sum ds0 k - c sum p k).  A single entry's ds is 0 (p is 1).
 template <typename T, int L>
 __global__ void __launch_bounds__(kBlock, kResident)
     neighbor_dq_kernel(const __grid_constant__ NeighborArgs a) {
   __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
   const Group<T, L> g(a, lists);
   const int at = g.j * Vec<T>::V;
-  Pairs<T> acc;
+  constexpr bool kRounded = sizeof(T) == 2;
+  Pairs<T> acc, mean;  // mean: sum p k
   acc.clear();
+  mean.clear();
+  float change = 0.f, first_dp = 0.f;
   uint4 q = make_uint4(0, 0, 0, 0), d = q;
   float part = 0.f;
   if (g.mine) {
@@ -305,8 +311,7 @@ __global__ void __launch_bounds__(kBlock, kResident)
     part = dot<T>(
         vector_at<T>(a.out, g.row * a.o_row + g.h * a.o_head + at), d);
   }
-  const float delta = group_sum<L>(part);
-  if (g.live && g.j == 0) a.delta[g.unit] = delta;
+  float delta = group_sum<L>(part);
   const float lse2 = g.live ? __ldg(a.lse + g.unit) * kLog2e : 0.f;
   uint4 ku[kAhead] = {}, vu[kAhead] = {};
   for (int j0 = 0; __any_sync(kFull, j0 < g.n); j0 += kAhead) {
@@ -316,9 +321,26 @@ __global__ void __launch_bounds__(kBlock, kResident)
       const float s = g.sum(dot<T>(ku[t], q));
       const float dp = g.sum(dot<T>(vu[t], d));
       const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2));
-      if (j0 + t < g.n) acc.add(p * (dp - delta), Pairs<T>(ku[t]));
+      if (j0 + t == 0) first_dp = dp;
+      if (j0 + t < g.n) {
+        const float ds = p * (dp - delta);
+        const Pairs<T> key(ku[t]);
+        acc.add(ds, key);
+        if constexpr (kRounded) {
+          mean.add(p, key);
+          change += ds;
+        }
+      }
     }
   }
+  if (g.n == 1) {
+    delta = first_dp;
+    acc.scale(first_dp - first_dp);
+  } else if constexpr (kRounded) {
+    delta += change;
+    acc.add(-change, mean);
+  }
+  if (g.live && g.j == 0) a.delta[g.unit] = delta;
   if (g.mine) {
     acc.scale(a.scale);
     *reinterpret_cast<uint4*>(static_cast<T*>(a.dq) + g.unit * a.dim + at) =

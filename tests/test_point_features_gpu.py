@@ -581,6 +581,70 @@ def test_cross_gradients_of_few_keys_beside_many(dim, dtype):
         assert torch.equal(got[: len(want)], want)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16), (24, FP16)])
+@pytest.mark.parametrize("kind", ["one", "masked", "beside"])
+def test_cross_gradients_of_a_single_key(kind, dim, dtype):
+    # one open key: its weight is 1 whatever the score, so dq and dk are 0
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    n_k = {"one": [1, 1], "masked": [7, 60], "beside": [1, 300]}[kind]
+    q, k, v, q_seg, k_seg = attention_inputs(200, ([140, 9], n_k), 4, 2, dim, dtype, scale=8.0)
+    mask = None
+    if kind == "masked":
+        mask = torch.zeros(67, dtype=torch.bool, device="cuda")
+        mask[[3, 66]] = True
+    check_cross(q, k, v, q_seg, k_seg, mask=mask)
+    pairs, d = ScenePairs(q_seg, k_seg), normal(201, *q.shape, dtype=dtype)
+    out, lse = cross_attention(q, k, v, pairs, mask=mask, return_lse=True)
+    dq, dk, dv = cross_attention_grad(d, q, k, v, out, lse, pairs, mask=mask)
+    whole = kind != "beside"
+    assert not dq[: None if whole else 140].any() and not dk[: None if whole else 1].any() and dv[:4].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("width,dim", [(1, 40), (9, 64), (32, 128)])
+def test_neighbor_gradients_of_a_single_key(width, dim, dtype):
+    from gsa_b200 import ScenePairs, neighbor_attention, neighbor_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(205, ([50, 3], [20, 6]), 4, 2, dim, dtype, scale=8.0)
+    ids = (torch.arange(53, device="cuda", dtype=torch.int32) % 6)[:, None].repeat(1, width)
+    pairs, d = ScenePairs(q_seg, k_seg), normal(206, *q.shape, dtype=dtype)
+    out, lse = neighbor_attention(q, k, v, ids, pairs, return_lse=True)
+    dq, dk, dv = neighbor_attention_grad(d, q, k, v, ids, out, lse, pairs)
+    assert not dq.any() and not dk.any() and dv.any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("entries", [2, 3, 8])
+def test_neighbor_gradients_do_not_see_the_outputs_rounding(entries, dtype):
+    from gsa_b200 import ScenePairs, neighbor_attention, neighbor_attention_grad
+
+    dim, n_k = 48, 40
+    q, k, v, q_seg, k_seg = attention_inputs(210, ([300], [n_k]), 2, 2, dim, dtype)
+    first = torch.arange(300, device="cuda")[:, None] * 7
+    ids = ((first + 3 * torch.arange(entries, device="cuda")) % n_k).int()
+    pairs, d = ScenePairs(q_seg, k_seg), normal(211, *q.shape, dtype=dtype)
+    out, lse = neighbor_attention(q, k, v, ids, pairs, return_lse=True)
+    dq, dk, _ = neighbor_attention_grad(d, q, k, v, ids, out, lse, pairs)
+    want = fo.Attention(q, k, v, q_seg, k_seg, ids=ids, dout=d)
+    Q, K, V, D = (t.double().cpu().transpose(0, 1) for t in (q, k, v, d))
+    count = fo.Attention.counts(ids.cpu().long(), n_k, True)
+    p = torch.softmax((Q @ K.mT * dim**-0.5).masked_fill(count == 0, -torch.inf), -1)
+    # Besides the result's own half step only 32-bit roundings: sums of 48
+    # products, below 2^-17 of the sums of magnitudes, in dp, delta and c, and
+    # in p and ds the scores' (below 2^-17 of |q| |k| / sqrt(dim) < 2^3) and
+    # lse's: 2^-13 of the magnitudes covers them, where bf16's `out` is rounded
+    # by 2^-9 and more of them and fp16's by 2^-12.
+    size = p * (D.abs() @ V.abs().mT + (D.abs() * (p @ V.abs())).sum(-1, keepdim=True))
+    half = torch.finfo(dtype).eps / 2
+    for got, exact, near in ((dq, want.dq, size @ K.abs()), (dk, want.dk, size.mT @ Q.abs())):
+        off = half * exact.abs() + 2.0**-13 * dim**-0.5 * near.transpose(0, 1) + 2.0**-25
+        error = (got.double().cpu() - exact).abs()
+        assert (error <= off).all(), float((error / off).max())
+        # and the errors together stay near the half step's alone
+        assert error.norm() <= 0.75 * half * exact.norm()
+
+
 @pytest.mark.parametrize("scale", [2.0**-24, 2.0**-12, 4.0])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_cross_scales(scale, dtype):
