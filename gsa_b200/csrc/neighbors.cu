@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kBlock, kResident)
   Pairs<T> acc, mean;  // mean: sum p k
   acc.clear();
   mean.clear();
-  float change = 0.f, first_dp = 0.f;
+  float change = 0.f;
   uint4 q = make_uint4(0, 0, 0, 0), d = q;
   float part = 0.f;
   if (g.mine) {
@@ -321,7 +321,6 @@ __global__ void __launch_bounds__(kBlock, kResident)
       const float s = g.sum(dot<T>(ku[t], q));
       const float dp = g.sum(dot<T>(vu[t], d));
       const float p = exp2_fast(fmaf(s, a.scale_log2e, -lse2));
-      if (j0 + t == 0) first_dp = dp;
       if (j0 + t < g.n) {
         const float ds = p * (dp - delta);
         const Pairs<T> key(ku[t]);
@@ -333,12 +332,16 @@ __global__ void __launch_bounds__(kBlock, kResident)
       }
     }
   }
-  if (g.n == 1) {
-    delta = first_dp;
-    acc.scale(first_dp - first_dp);
-  } else if constexpr (kRounded) {
+  if constexpr (kRounded) {
     delta += change;
     acc.add(-change, mean);
+  }
+  if (__any_sync(kFull, g.n == 1)) {
+    const float dp = g.sum(dot<T>(vu[0], d));  // of the first entry, if single
+    if (g.n == 1) {
+      delta = dp;
+      acc.scale(dp - dp);
+    }
   }
   if (g.live && g.j == 0) a.delta[g.unit] = delta;
   if (g.mine) {
