@@ -614,7 +614,8 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         const float f = which ? power_of_two(-p_bits<T>())
                               : a.scale * power_of_two(-bits);
         T* out = static_cast<T*>(kKeysPass ? (which ? a.dv : a.dk) : a.dq) + at;
-        float* sum = a.part + ((kKeysPass ? 2 : 1) * split + which) * parts + at;
+        float* sum =
+            a.part + ((kKeysPass ? 2 : 1) * split + which) * parts + at;
         for (int i = part * 8; i < a.dim; i += 8 * S::kShare) {
           uint32_t x[8];
           float y[8];

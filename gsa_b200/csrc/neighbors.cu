@@ -27,8 +27,8 @@
 // result (397 us for 388 forward, 488 for 464 forward and back).
 //
 // 192,000 rows of 32 entries, 8 heads of 32 in bf16: 388 us, 1.08 TB/s of
-// tensors in device memory (418 MB) and 12 TB/s of gathered heads through L1 and
-// L2.  48,000 rows, 4 heads of 32 in FP32, forward and back: 464 us, of them
+// tensors in device memory (418 MB) and 12 TB/s of gathered heads through L1
+// and L2.  48,000 rows, 4 heads of 32 in FP32, forward and back: 462 us, of them
 // about 105 forward, 95 for the order of the entries, 110 for dq and 185 for dk
 // and dv.
 #include "features.cuh"
@@ -151,7 +151,8 @@ __device__ __forceinline__ uint4 gather(const void* base, int row,
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 vector_at(const void* base, long long element) {
+__device__ __forceinline__ uint4 vector_at(const void* base,
+                                           long long element) {
   return __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) +
                                               element));
 }
@@ -292,8 +293,10 @@ __global__ void __launch_bounds__(kBlock, kResident)
 // `out` would be most of the error of ds, so that <dout, out> only serves as a
 // start d0 there: with ds0 = p (dp - d0) and c = sum ds0, delta = d0 + c and
 // dq = scale (sum ds0 k - c sum p k).  A single entry's ds is 0 (p is 1).
+// The further sum costs registers: 48,000 rows in bf16, forward and back, with
+// 7 blocks on an SM 396 us, with 8 (spills) 416, with 6 403.
 template <typename T, int L>
-__global__ void __launch_bounds__(kBlock, kResident)
+__global__ void __launch_bounds__(kBlock, sizeof(T) == 2 ? 7 : kResident)
     neighbor_dq_kernel(const __grid_constant__ NeighborArgs a) {
   __shared__ __align__(16) RowLists<kBlock / L + 1> lists;
   const Group<T, L> g(a, lists);
