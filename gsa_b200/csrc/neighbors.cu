@@ -29,7 +29,7 @@
 // 192,000 rows of 32 entries, 8 heads of 32 in bf16: 388 us, 1.08 TB/s of
 // tensors in device memory (418 MB) and 12 TB/s of gathered heads through L1
 // and L2.  48,000 rows, 4 heads of 32 in FP32, forward and back: 462 us, of them
-// about 105 forward, 95 for the order of the entries, 110 for dq and 185 for dk
+// about 98 forward, 87 for the order of the entries, 103 for dq and 173 for dk
 // and dv.
 #include "features.cuh"
 #include "tensor_core.cuh"

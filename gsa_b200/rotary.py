@@ -122,7 +122,8 @@ class Rotary:
         """The rows ``x`` (FP32, FP16 or BF16 (N, heads, dim), any row and
         head strides) turned by ``positions`` (FP32, int32 or int64
         (N, axes), or (N,) for one axis).  ``out`` may be ``x`` itself, else it does not
-        overlap it.  Differentiable in ``x`` unless ``out`` is given."""
+        overlap it.  Differentiable in ``x`` unless ``out`` is given; in a
+        captured graph, take the gradient by ``grad``."""
         if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
             if out is not None:
                 raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
