@@ -9,8 +9,8 @@ place in an order (``axes`` = 1), where ``scaling`` extends a network to
 longer orders than it was trained on.
 """
 
-import ctypes
 import math
+from array import array
 
 import torch
 
@@ -77,8 +77,8 @@ class Rotary:
         self.pairs = part // (2 * axes)
         self._interleaved = layout == "interleaved"
         f = frequencies(self.pairs, base, scaling, factor, length)
-        self._turns = (ctypes.c_double * self.pairs)(*[v / (2 * math.pi) / unit for v in f])
-        self._turns_at = ctypes.addressof(self._turns)
+        # copied and pickled with the plan, so its address is asked for per call
+        self._turns = array("d", [v / (2 * math.pi) / unit for v in f])
 
     def _run(self, x, positions, out, transposed):
         try:
@@ -111,7 +111,7 @@ class Rotary:
         steps = positions.stride()
         args = ft.pack_rotary(
             ft.TYPES[dtype], rows, heads, dim, *place, *to, positions.data_ptr(), kind, steps[0], steps[1] if axes else 0,
-            self.axes, self.pairs, self._turns_at, self.amplitude, self._interleaved, transposed, stream,
+            self.axes, self.pairs, self._turns.buffer_info()[0], self.amplitude, self._interleaved, transposed, stream,
         )
         code = ft.lib.rotary_positions(args)
         if code:

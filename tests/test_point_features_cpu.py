@@ -3,10 +3,15 @@
 entries and the Python calls refuse before any launch, the frequency tables
 and the oracle's own gradients."""
 
+import copy
 import ctypes
+import gc
 import math
+import pickle
 import re
+import struct
 import subprocess
+import types
 from pathlib import Path
 
 import pytest
@@ -228,3 +233,35 @@ def test_oracle_gradients_are_those_of_its_output():
                    for s in (1, -1)]
             got = (two[0] - two[1]) / (2 * h)
             assert torch.isclose(got, (getattr(o, name) * step).sum(), rtol=1e-6, atol=1e-8), (kw, name)
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that passes for one of device 0."""
+
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def test_copies_of_a_rotary_plan_have_turns_of_their_own(monkeypatch):
+    plan = Rotary(20, axes=2, base=500.0, unit=0.5)
+    want, seen = list(plan._turns), []
+
+    def entry(args):
+        at = struct.unpack_from("=17q", args)[16]
+        seen.append(list((ctypes.c_double * plan_pairs).from_address(at)))
+        return 0
+
+    plan_pairs = plan.pairs
+    copies = [copy.copy(plan), copy.deepcopy(plan), copy.deepcopy(copy.deepcopy(plan)), pickle.loads(pickle.dumps(plan))]
+    del plan
+    gc.collect()
+    others = [(ctypes.c_double * plan_pairs)(*[7.0] * plan_pairs) for _ in range(500)]
+    monkeypatch.setattr(rotary, "current_stream", lambda: (0, 0))
+    monkeypatch.setattr(ft, "lib", types.SimpleNamespace(rotary_positions=entry))
+    x, y = (torch.zeros(4, 2, 24).as_subclass(OnDevice) for _ in range(2))
+    place = torch.zeros(4, 2).as_subclass(OnDevice)
+    for twin in copies:
+        twin(x, place, out=y)
+    assert seen == [want] * 4 and len(others) == 500
