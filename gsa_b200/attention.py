@@ -32,7 +32,8 @@ class ScenePairs:
 
     Offsets start at 0, never fall (a scene may have no queries or no keys)
     and end at the number of rows.  They are uploaded once; make the object
-    outside a graph capture, and keep it as long as graphs that used it."""
+    outside a graph capture, and keep it as long as graphs that used it.  A copy
+    of it, or one from a pickle, is uploaded anew."""
 
     def __init__(self, q_seg, k_seg):
         q_seg, k_seg = [int(v) for v in q_seg], [int(v) for v in k_seg]
@@ -52,6 +53,10 @@ class ScenePairs:
         self._k_at = self._q_at + 4 * len(q_seg)
         self._error_at = self._k_at + 4 * len(k_seg)
 
+    def __reduce__(self):
+        # a copy, or an unpickled one, has offsets and a flag of its own
+        return _pairs_on, (self.device, type(self), self.q_seg, self.k_seg)
+
     @classmethod
     def of_lengths(cls, queries, keys):
         """From the scenes' numbers of query and of key rows."""
@@ -62,6 +67,11 @@ class ScenePairs:
         these pairs (their results are then void).  Synchronises."""
         if int(self._ints[-1]):
             raise RuntimeError("cross attention: a wait for the tensor cores ran out")
+
+
+def _pairs_on(device, kind, q_seg, k_seg):
+    with torch.cuda.device(device):
+        return kind(q_seg, k_seg)
 
 
 class _Call:

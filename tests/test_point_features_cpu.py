@@ -3,6 +3,7 @@
 entries and the Python calls refuse before any launch, the frequency tables
 and the oracle's own gradients."""
 
+import contextlib
 import copy
 import ctypes
 import gc
@@ -265,3 +266,15 @@ def test_copies_of_a_rotary_plan_have_turns_of_their_own(monkeypatch):
     for twin in copies:
         twin(x, place, out=y)
     assert seen == [want] * 4 and len(others) == 500
+
+
+def test_copies_of_scene_pairs_have_offsets_of_their_own(monkeypatch):
+    monkeypatch.setattr(attention, "current_stream", lambda: (0, 0))
+    monkeypatch.setattr(torch.cuda, "device", lambda _: contextlib.nullcontext())
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, *_, **__: t.clone())
+    pairs = ScenePairs([0, 3, 7], [0, 5, 5])
+    for twin in (copy.copy(pairs), copy.deepcopy(pairs), pickle.loads(pickle.dumps(pairs))):
+        assert (twin.q_seg, twin.k_seg, twin.device) == (pairs.q_seg, pairs.k_seg, 0)
+        at = twin._ints.data_ptr()
+        assert at != pairs._ints.data_ptr() and twin._ints.tolist() == [0, 3, 7, 0, 5, 5, 0]
+        assert (twin._q_at, twin._k_at, twin._error_at) == (at, at + 12, at + 24)

@@ -3,7 +3,10 @@
 64-bit oracles (``tests/features_oracle.py``, whose bounds are derived there),
 and the ways a program calls them."""
 
+import copy
+import gc
 import math
+import pickle
 
 import pytest
 import torch
@@ -756,3 +759,20 @@ def test_attention_refuses():
             at.cross_attention_grad(**args)
         with pytest.raises(ValueError):
             at.neighbor_attention_grad(rows=ids, **args)
+
+
+def test_copies_and_pickles_outlive_their_originals():
+    from gsa_b200 import Rotary, ScenePairs, cross_attention
+
+    q, k, v, q_seg, k_seg = attention_inputs(300, ([70, 3], [200, 60]), 2, 2, 32, BF16)
+    place = normal(301, 73, 3)
+    r, pairs = Rotary(30, axes=3), ScenePairs(q_seg, k_seg)
+    turned, want = r(q, place), cross_attention(q, k, v, pairs)
+    copies = [(copy.deepcopy(r), copy.deepcopy(pairs)), (copy.copy(r), copy.copy(pairs)), pickle.loads(pickle.dumps((r, pairs)))]
+    del r, pairs
+    gc.collect()
+    later = [torch.full((7,), -1, dtype=torch.int32, device="cuda") for _ in range(64)]
+    for turn, twin in copies:
+        assert torch.equal(turn(q, place), turned) and torch.equal(cross_attention(q, k, v, twin), want)
+        twin.check()
+    assert len(later) == 64
