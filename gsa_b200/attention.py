@@ -278,10 +278,11 @@ def neighbor_attention_grad(dout, q, k, v, rows, out, lse, pairs, padded=True, s
 
 def _vectors(t):
     """A gradient as the kernels take it (autograd may hand over an expanded
-    or otherwise laid out one)."""
+    or otherwise laid out one, or one that starts anywhere: a contiguous view
+    behind other columns, say, of which ``contiguous()`` makes no copy)."""
     size = t.element_size()
     fits = t.stride(2) == 1 and not (t.data_ptr() | t.stride(0) * size | t.stride(1) * size) & 15
-    return t if fits else t.contiguous()
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 
 class _Cross(torch.autograd.Function):

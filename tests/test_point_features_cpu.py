@@ -278,3 +278,11 @@ def test_copies_of_scene_pairs_have_offsets_of_their_own(monkeypatch):
         at = twin._ints.data_ptr()
         assert at != pairs._ints.data_ptr() and twin._ints.tolist() == [0, 3, 7, 0, 5, 5, 0]
         assert (twin._q_at, twin._k_at, twin._error_at) == (at, at + 12, at + 24)
+
+
+def test_gradients_are_laid_out_for_the_kernels():
+    flat = torch.randn(3 + 2 * 64).to(torch.bfloat16)
+    for t in (flat[3:].view(2, 2, 32), flat[3:67].view(1, 2, 32), flat[:128].view(2, 2, 32), flat[:64].view(1, 2, 32).expand(3, 2, 32),
+              flat[:128].view(2, 32, 2).transpose(1, 2)):
+        got = attention._vectors(t)
+        assert torch.equal(got, t) and got.data_ptr() % 16 == 0 and got.stride(2) == 1

@@ -776,3 +776,24 @@ def test_copies_and_pickles_outlive_their_originals():
         assert torch.equal(turn(q, place), turned) and torch.equal(cross_attention(q, k, v, twin), want)
         twin.check()
     assert len(later) == 64
+
+
+@pytest.mark.parametrize("kind", ["cross", "neighbor"])
+def test_gradients_that_start_anywhere(kind):
+    # one row behind three columns, and a view into a flat buffer: contiguous
+    # as torch counts, but not on 16 bytes
+    for lengths in (([1], [70]), ([130, 64], [70, 129])):
+        leaves, d, forward, backward = both(kind, lengths)
+        out, lse = forward(return_lse=True)
+        want = backward(out, lse)
+        for t in leaves:
+            t.requires_grad_()
+        n = len(d)
+        torch.cat((d.new_zeros(n, 3), forward().flatten(1)), 1).backward(torch.cat((d.new_ones(n, 3), d.flatten(1)), 1))
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+        for t in leaves:
+            t.grad = None
+        flat = torch.cat((d.new_zeros(1), d.flatten()))[1:].view_as(d)
+        assert flat.is_contiguous() and flat.data_ptr() % 16
+        forward().backward(flat)
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
