@@ -9,6 +9,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from ._library import load
 
@@ -37,6 +38,15 @@ def check(code, what):
         raise ValueError(f"{what}: sizes or strides out of range")
     if code:
         raise RuntimeError(f"{what}: CUDA error {code}")
+
+
+def check_tangents(*tensors):
+    """Within a forward-mode level, none of the inputs carries a tangent: the
+    kernels would drop it."""
+    if forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors
+    ):
+        raise ValueError("the operators on points' features have no forward-mode derivatives")
 
 
 def rows_of(t, what, shape, dtype, device):

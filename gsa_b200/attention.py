@@ -200,6 +200,7 @@ _ALL = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _wants_grad(out, *tensors):
+    ft.check_tangents(*tensors)
     if not (any(getattr(t, "requires_grad", False) for t in tensors) and torch.is_grad_enabled()):
         return False
     if out is not None:
@@ -239,6 +240,7 @@ def cross_attention_grad(dout, q, k, v, out, lse, pairs, mask=None, scale=None):
     """``(dq, dk, dv)`` from the gradient of ``cross_attention``'s ``out``;
     the other arguments are that call's, with its ``out`` and ``lse``.  The
     sums have a fixed order: the same arguments give the same bits."""
+    ft.check_tangents(dout, q, k, v, out, lse)
     call = _Call("cross attention gradient", q, k, v, pairs, scale, _HALF)
     call.set_mask(mask)
     return call.backward(ft.lib.cross_attention_grad, ft.lib.cross_attention_grad_workspace, dout, out, lse)
@@ -271,6 +273,7 @@ def neighbor_attention(q, k, v, rows, pairs, padded=True, scale=None, out=None, 
 def neighbor_attention_grad(dout, q, k, v, rows, out, lse, pairs, padded=True, scale=None):
     """``(dq, dk, dv)`` from the gradient of ``neighbor_attention``'s
     ``out``, in a fixed order of sums like ``cross_attention_grad``."""
+    ft.check_tangents(dout, q, k, v, out, lse)
     call = _Call("neighbor attention gradient", q, k, v, pairs, scale, _ALL)
     call.set_ids(rows, padded)
     return call.backward(ft.lib.neighbor_attention_grad, ft.lib.neighbor_attention_grad_workspace, dout, out, lse)

@@ -124,6 +124,7 @@ class Rotary:
         (N, axes), or (N,) for one axis).  ``out`` may be ``x`` itself, else it does not
         overlap it.  Differentiable in ``x`` unless ``out`` is given; in a
         captured graph, take the gradient by ``grad``."""
+        ft.check_tangents(x, positions)
         if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
             if out is not None:
                 raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
@@ -132,6 +133,7 @@ class Rotary:
 
     def grad(self, dy, positions, out=None):
         """The gradient of ``x`` from that of ``rotary(x, positions)``."""
+        ft.check_tangents(dy, positions)
         return self._run(dy, positions, out, True)
 
 

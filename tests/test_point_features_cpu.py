@@ -17,6 +17,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import gsa_b200
 from gsa_b200 import ScenePairs, Rotary, _features as ft, _library, attention, rotary
@@ -286,3 +287,19 @@ def test_gradients_are_laid_out_for_the_kernels():
               flat[:128].view(2, 32, 2).transpose(1, 2)):
         got = attention._vectors(t)
         assert torch.equal(got, t) and got.data_ptr() % 16 == 0 and got.stride(2) == 1
+
+
+def test_calls_refuse_forward_mode_derivatives():
+    x = torch.zeros(4, 2, 16)
+    place, ids, lse = torch.zeros(4), torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4, 2)
+    turn = Rotary(16)
+    with forward_ad.dual_level():
+        moved, moved_place = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(place, torch.ones_like(place))
+        for call in (lambda: turn(moved, place), lambda: turn.grad(moved, place), lambda: turn(x, moved_place),
+                     lambda: turn(moved, place, out=x),
+                     lambda: attention.cross_attention(x, moved, x, None), lambda: attention.cross_attention(moved, x, x, None, out=x),
+                     lambda: attention.neighbor_attention(x, x, moved, ids, None),
+                     lambda: attention.cross_attention_grad(moved, x, x, x, x, lse, None),
+                     lambda: attention.neighbor_attention_grad(x, x, moved, x, ids, x, lse, None)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
