@@ -118,13 +118,19 @@ class Rotary:
             ft.check(code, "rotary positions")
         return out
 
+    @staticmethod
+    def _check_derivatives(x, positions):
+        ft.check_tangents(x, positions)
+        if getattr(positions, "requires_grad", False) and torch.is_grad_enabled():
+            raise ValueError("positions get no gradient: detach them, or call under torch.no_grad()")
+
     def __call__(self, x, positions, out=None):
         """The rows ``x`` (FP32, FP16 or BF16 (N, heads, dim), any row and
         head strides) turned by ``positions`` (FP32, int32 or int64
         (N, axes), or (N,) for one axis).  ``out`` may be ``x`` itself, else it does not
-        overlap it.  Differentiable in ``x`` unless ``out`` is given; in a
-        captured graph, take the gradient by ``grad``."""
-        ft.check_tangents(x, positions)
+        overlap it.  Differentiable in ``x`` unless ``out`` is given, not in
+        the positions; in a captured graph, take the gradient by ``grad``."""
+        self._check_derivatives(x, positions)
         if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
             if out is not None:
                 raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
@@ -133,7 +139,7 @@ class Rotary:
 
     def grad(self, dy, positions, out=None):
         """The gradient of ``x`` from that of ``rotary(x, positions)``."""
-        ft.check_tangents(dy, positions)
+        self._check_derivatives(dy, positions)
         return self._run(dy, positions, out, True)
 
 

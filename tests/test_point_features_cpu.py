@@ -303,3 +303,13 @@ def test_calls_refuse_forward_mode_derivatives():
                      lambda: attention.neighbor_attention_grad(x, x, moved, x, ids, x, lse, None)):
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
+
+
+def test_rotary_refuses_positions_that_want_a_gradient():
+    x, place = torch.zeros(4, 2, 16), torch.zeros(4).requires_grad_()
+    leaf, turn = x.clone().requires_grad_(), Rotary(16)
+    for call in (lambda: turn(x, place), lambda: turn.grad(x, place), lambda: turn(leaf, place), lambda: turn(x, place, out=x)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="rows must be CUDA"):
+            call()
