@@ -118,11 +118,16 @@ class Rotary:
             ft.check(code, "rotary positions")
         return out
 
-    @staticmethod
-    def _check_derivatives(x, positions):
+    def _turn(self, x, positions, out, transposed):
         ft.check_tangents(x, positions)
-        if getattr(positions, "requires_grad", False) and torch.is_grad_enabled():
-            raise ValueError("positions get no gradient: detach them, or call under torch.no_grad()")
+        if torch.is_grad_enabled():
+            if getattr(positions, "requires_grad", False):
+                raise ValueError("positions get no gradient: detach them, or call under torch.no_grad()")
+            if getattr(x, "requires_grad", False):
+                if out is not None:
+                    raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
+                return _Turn.apply(x, positions, self, transposed)
+        return self._run(x, positions, out, transposed)
 
     def __call__(self, x, positions, out=None):
         """The rows ``x`` (FP32, FP16 or BF16 (N, heads, dim), any row and
@@ -130,30 +135,24 @@ class Rotary:
         (N, axes), or (N,) for one axis).  ``out`` may be ``x`` itself, else it does not
         overlap it.  Differentiable in ``x`` unless ``out`` is given, not in
         the positions; in a captured graph, take the gradient by ``grad``."""
-        self._check_derivatives(x, positions)
-        if getattr(x, "requires_grad", False) and torch.is_grad_enabled():
-            if out is not None:
-                raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
-            return _Turn.apply(x, positions, self)
-        return self._run(x, positions, out, False)
+        return self._turn(x, positions, out, False)
 
     def grad(self, dy, positions, out=None):
-        """The gradient of ``x`` from that of ``rotary(x, positions)``."""
-        self._check_derivatives(dy, positions)
-        return self._run(dy, positions, out, True)
+        """The gradient of ``x`` from that of ``rotary(x, positions)``; linear
+        in ``dy`` and differentiable in it as ``rotary`` is in ``x``."""
+        return self._turn(dy, positions, out, True)
 
 
 class _Turn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, positions, rotary):
+    def forward(ctx, x, positions, rotary, transposed):
         ctx.save_for_backward(positions)
-        ctx.rotary = rotary
-        return rotary._run(x, positions, None, False)
+        ctx.rotary, ctx.transposed = rotary, transposed
+        return rotary._run(x, positions, None, transposed)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         (positions,) = ctx.saved_tensors
         if dy.stride(2) != 1:
             dy = dy.contiguous()
-        return ctx.rotary._run(dy, positions, None, True), None, None
+        return ctx.rotary._turn(dy, positions, None, not ctx.transposed), None, None, None

@@ -797,3 +797,21 @@ def test_gradients_that_start_anywhere(kind):
         assert flat.is_contiguous() and flat.data_ptr() % 16
         forward().backward(flat)
         assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+
+
+def test_rotary_gradients_have_gradients():
+    from gsa_b200 import Rotary
+
+    r = Rotary(30, axes=3, layout="interleaved", amplitude=1.5)
+    place = normal(321, 40, 3)
+    d, e = normal(322, 40, 2, 32).requires_grad_(), normal(323, 40, 2, 32)
+    r.grad(d, place).backward(e)  # linear in d, its gradient the turn itself
+    assert torch.equal(d.grad, r(e, place))
+    x = normal(324, 40, 2, 32).requires_grad_()
+    d = d.detach().requires_grad_()
+    (dx,) = torch.autograd.grad(r(x, place), x, d, create_graph=True)
+    assert torch.equal(dx, r.grad(d.detach(), place))
+    dx.backward(e)
+    assert torch.equal(d.grad, r(e, place)) and x.grad is None
+    with pytest.raises(ValueError):
+        r.grad(d, place, out=torch.empty_like(e))
