@@ -208,6 +208,14 @@ def _wants_grad(out, *tensors):
     return True
 
 
+def _no_second(dout, *others):
+    """A gradient call on a ``dout`` that autograd follows would end its
+    derivatives in silence."""
+    ft.check_tangents(dout, *others)
+    if getattr(dout, "requires_grad", False) and torch.is_grad_enabled():
+        raise ValueError("attention has no second derivatives: detach dout, or call under torch.no_grad()")
+
+
 def _cross(q, k, v, pairs, mask, scale, out, return_lse):
     call = _Call("cross attention", q, k, v, pairs, scale, _HALF)
     call.set_mask(mask)
@@ -239,8 +247,9 @@ def cross_attention(q, k, v, pairs, mask=None, scale=None, out=None, return_lse=
 def cross_attention_grad(dout, q, k, v, out, lse, pairs, mask=None, scale=None):
     """``(dq, dk, dv)`` from the gradient of ``cross_attention``'s ``out``;
     the other arguments are that call's, with its ``out`` and ``lse``.  The
-    sums have a fixed order: the same arguments give the same bits."""
-    ft.check_tangents(dout, q, k, v, out, lse)
+    sums have a fixed order: the same arguments give the same bits.  The
+    results take no part in autograd."""
+    _no_second(dout, q, k, v, out, lse)
     call = _Call("cross attention gradient", q, k, v, pairs, scale, _HALF)
     call.set_mask(mask)
     return call.backward(ft.lib.cross_attention_grad, ft.lib.cross_attention_grad_workspace, dout, out, lse)
@@ -272,8 +281,9 @@ def neighbor_attention(q, k, v, rows, pairs, padded=True, scale=None, out=None, 
 
 def neighbor_attention_grad(dout, q, k, v, rows, out, lse, pairs, padded=True, scale=None):
     """``(dq, dk, dv)`` from the gradient of ``neighbor_attention``'s
-    ``out``, in a fixed order of sums like ``cross_attention_grad``."""
-    ft.check_tangents(dout, q, k, v, out, lse)
+    ``out``, in a fixed order of sums and outside autograd like
+    ``cross_attention_grad``."""
+    _no_second(dout, q, k, v, out, lse)
     call = _Call("neighbor attention gradient", q, k, v, pairs, scale, _ALL)
     call.set_ids(rows, padded)
     return call.backward(ft.lib.neighbor_attention_grad, ft.lib.neighbor_attention_grad_workspace, dout, out, lse)

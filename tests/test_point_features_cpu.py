@@ -313,3 +313,14 @@ def test_rotary_refuses_positions_that_want_a_gradient():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="rows must be CUDA"):
             call()
+
+
+def test_attention_gradients_refuse_to_be_differentiated():
+    x, lse = torch.zeros(4, 2, 16), torch.zeros(4, 2)
+    ids, leaf = torch.zeros(4, 3, dtype=torch.int32), x.clone().requires_grad_()
+    for call in (lambda: attention.cross_attention_grad(leaf, x, x, x, x, lse, None),
+                 lambda: attention.neighbor_attention_grad(leaf, x, x, x, ids, x, lse, None)):
+        with pytest.raises(ValueError, match="second derivatives"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="needs CUDA"):
+            call()
