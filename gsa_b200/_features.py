@@ -49,6 +49,13 @@ def check_tangents(*tensors):
         raise ValueError("the operators on points' features have no forward-mode derivatives")
 
 
+def check_outside_autograd(out, *tensors):
+    """With gradients enabled, a call that writes ``out`` neither reads nor
+    writes what autograd follows."""
+    if out is not None and any(getattr(t, "requires_grad", False) for t in (out, *tensors)):
+        raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
+
+
 def rows_of(t, what, shape, dtype, device):
     """``(data, row stride, head stride)`` of a CUDA tensor of rows of heads;
     anything but the expected shape, type and device raises."""

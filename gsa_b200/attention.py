@@ -201,11 +201,10 @@ _ALL = (torch.float32, torch.bfloat16, torch.float16)
 
 def _wants_grad(out, *tensors):
     ft.check_tangents(*tensors)
-    if not (any(getattr(t, "requires_grad", False) for t in tensors) and torch.is_grad_enabled()):
+    if not torch.is_grad_enabled():
         return False
-    if out is not None:
-        raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
-    return True
+    ft.check_outside_autograd(out, *tensors)
+    return any(getattr(t, "requires_grad", False) for t in tensors)
 
 
 def _no_second(dout, *others):

@@ -123,9 +123,8 @@ class Rotary:
         if torch.is_grad_enabled():
             if getattr(positions, "requires_grad", False):
                 raise ValueError("positions get no gradient: detach them, or call under torch.no_grad()")
+            ft.check_outside_autograd(out, x)
             if getattr(x, "requires_grad", False):
-                if out is not None:
-                    raise ValueError("a call with out= takes no part in autograd: give none, or call under torch.no_grad()")
                 return _Turn.apply(x, positions, self, transposed)
         return self._run(x, positions, out, transposed)
 

@@ -324,3 +324,14 @@ def test_attention_gradients_refuse_to_be_differentiated():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="needs CUDA"):
             call()
+
+
+def test_written_tensors_that_autograd_follows_are_refused():
+    x, place, ids = torch.zeros(4, 2, 16), torch.zeros(4), torch.zeros(4, 3, dtype=torch.int32)
+    out, turn = x.clone().requires_grad_(), Rotary(16)
+    for call in (lambda: turn(x, place, out=out), lambda: turn.grad(x, place, out=out),
+                 lambda: attention.cross_attention(x, x, x, None, out=out), lambda: attention.neighbor_attention(x, x, x, ids, None, out=out)):
+        with pytest.raises(ValueError, match="takes no part in autograd"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            call()
