@@ -4,7 +4,8 @@
 //
 //   s = scale q k^T,  out = softmax(s) v,  lse = log sum exp s,
 //
-// over the scene's open keys; a row without any gives 0 and lse = -inf.
+// over the scene's open keys; a row without any gives 0 and lse = -inf, one
+// whose scores are all -inf has no softmax and gives NaN for both.
 //
 // A block owns 128 packed query rows, a row per thread, and walks the keys in
 // tiles of 128.  A fifth warp issues the products (tcgen05), a sixth loads the
@@ -377,7 +378,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (a.splits > 1)
           a.part_lse[at] = seen && none ? -3.0e38f : lse2;
         else if (a.lse)
-          a.lse[at] = lse2 * kLn2;
+          a.lse[at] =
+              seen && l == 0.f ? __int_as_float(0x7fffffff) : lse2 * kLn2;
       }
       if (a.splits == 1) {
         // Through Q's place (its products are complete), so that whole rows

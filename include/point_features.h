@@ -89,7 +89,8 @@ typedef struct {
 
 /* out = softmax(scale q k^T) v over the open keys of each query's scene, for
  * float16 and bfloat16; lse = log sum exp of the scores.  A row without open
- * keys gives 0 and lse = -inf.  Shut keys may hold anything.
+ * keys gives 0 and lse = -inf; one of open keys whose scores are all -inf gives
+ * NaN and lse = NaN.  Shut keys may hold anything.
  * The workspace calls read the sizes only and return bytes, or -2. */
 int cross_attention(const attention_args* a);
 int64_t cross_attention_workspace(const attention_args* a);

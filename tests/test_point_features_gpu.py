@@ -815,3 +815,21 @@ def test_rotary_gradients_have_gradients():
     assert torch.equal(d.grad, r(e, place)) and x.grad is None
     with pytest.raises(ValueError):
         r.grad(d, place, out=torch.empty_like(e))
+
+
+@pytest.mark.parametrize("n_k", [60, 400, 3000])
+def test_cross_rows_of_minus_infinity_have_no_gradients(n_k):
+    # no softmax: NaN, which the gradient's weights have too, in one part and
+    # in several
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(310, ([6, 4], [n_k, 5]), 1, 1, 32, BF16)
+    q[:6], k[:n_k] = 1.0, 0.0
+    k[:n_k, 0, 0] = -math.inf
+    pairs, d = ScenePairs(q_seg, k_seg), normal(311, *q.shape, dtype=BF16)
+    out, lse = cross_attention(q, k, v, pairs, return_lse=True)
+    assert out[:6].isnan().all() and lse[:6].isnan().all()
+    assert out[6:].isfinite().all() and lse[6:].isfinite().all()
+    dq, dk, dv = cross_attention_grad(d, q, k, v, out, lse, pairs)
+    assert dq[:6].isnan().all() and dk[:n_k].isnan().all() and dv[:n_k].isnan().all()
+    assert dq[6:].isfinite().all() and dk[n_k:].isfinite().all() and dv[n_k:].isfinite().all()
