@@ -64,7 +64,9 @@ class ScenePairs:
 
     def check(self):
         """Raise if a kernel's bounded wait ran out in any call so far with
-        these pairs (their results are then void).  Synchronises."""
+        these pairs, on whichever stream (their results are then void).
+        Synchronises the device."""
+        torch.cuda.synchronize(self.device)
         if int(self._ints[-1]):
             raise RuntimeError("cross attention: a wait for the tensor cores ran out")
 

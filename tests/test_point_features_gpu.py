@@ -833,3 +833,25 @@ def test_cross_rows_of_minus_infinity_have_no_gradients(n_k):
     dq, dk, dv = cross_attention_grad(d, q, k, v, out, lse, pairs)
     assert dq[:6].isnan().all() and dk[:n_k].isnan().all() and dv[:n_k].isnan().all()
     assert dq[6:].isfinite().all() and dk[n_k:].isfinite().all() and dv[n_k:].isfinite().all()
+
+
+def test_the_error_flag_of_another_stream_is_waited_for():
+    from gsa_b200 import ScenePairs
+
+    pairs = ScenePairs([0, 4], [0, 4])
+    pairs.check()
+    x, side = normal(330, 4096, 4096), torch.cuda.Stream()
+
+    def late(flag, times):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(times):  # some milliseconds before the flag is set
+                x @ x
+            flag.fill_(1)
+
+    late(torch.zeros(1, dtype=torch.int32, device="cuda"), 1)  # kernels loaded
+    torch.cuda.synchronize()
+    late(pairs._ints[-1:], 40)
+    assert not side.query()
+    with pytest.raises(RuntimeError):
+        pairs.check()
