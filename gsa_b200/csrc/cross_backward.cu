@@ -127,29 +127,43 @@ __device__ __forceinline__ void product_more(uint32_t d, uint32_t a,
           tc::instruction<T>(kN, false), true);
 }
 
-// kFew (queries' pass): scenes may have their keys in one tile.
-template <typename T, int kDim, bool kKeysPass, bool kFew>
-__global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
-                                  Shape<kDim, kKeysPass>::kBlocks)
-    cross_backward_kernel(const __grid_constant__ CrossArgs a,
-                          const __grid_constant__ BackMaps maps) {
+// Whether one of n keys is open and no more.  By a whole warp.
+__device__ __forceinline__ bool single_key(const unsigned char* mask, int n) {
+  if (!mask) return n == 1;
+  int open = 0;
+  for (int k = threadIdx.x & 31; open < 2 && k - (int)(threadIdx.x & 31) < n;
+       k += 8 * 32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      open += __popc(__ballot_sync(
+          kFull, k + i * 32 < n && __ldg(mask + k + i * 32)));
+  }
+  return open == 1;
+}
+
+// What the warps of a block share besides the tiles.
+template <typename S, bool kKeysPass>
+struct Shared {
+  uint64_t bars[kBars];
+  uint32_t tmem_at;
+  float part_delta[kKeysPass ? 1 : S::kShare][kKeysPass ? 1 : kRows];
+};
+
+// A block's work: rows from r0 on of a scene (n packed rows from q0 on, nk keys
+// from k0 on) and of one head of keys, one share of the walked ones.  kOneTile
+// (queries' pass): the scene's keys are in one tile; then delta is the sum of P *
+// dP, without the rounding of `out`, which would be most of dS's error where
+// keys are few.
+template <typename T, int kDim, bool kKeysPass, bool kOneTile>
+__device__ __forceinline__ void backward_block(
+    const CrossArgs& a, const BackMaps& maps,
+    Shared<Shape<kDim, kKeysPass>, kKeysPass>& shared, int q0, int n, int k0,
+    int nk, int hk, int split, int r0) {
   using S = Shape<kDim, kKeysPass>;
   constexpr int W = S::kWalk, kRowWarps = S::kRowWarps;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[kBars];
-  __shared__ uint32_t tmem_at;
-  __shared__ float part_delta[S::kShare][kRows];
+  auto& part_delta = shared.part_delta;
 
-  unsigned unit = blockIdx.x;
-  const int r0 = unit % a.tiles * kRows;
-  unit /= a.tiles;
-  const int split = unit % a.splits;
-  unit /= a.splits;
-  const int hk = unit % a.kv_heads;
-  const int scene = unit / a.kv_heads;
-  const int q0 = __ldg(a.q_seg + scene), k0 = __ldg(a.k_seg + scene);
-  const int n = (__ldg(a.q_seg + scene + 1) - q0) * a.group;  // packed rows
-  const int nk = __ldg(a.k_seg + scene + 1) - k0;
   const int own = kKeysPass ? nk : n, walked = kKeysPass ? n : nk;
   // a walked tile of packed rows holds whole query rows
   const int each = kKeysPass ? W / a.group * a.group : W;
@@ -157,9 +171,6 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
   int begin, end;
   share((walked + each - 1) / each, a.splits, split, &begin, &end);
   const int nt = end - begin;
-  // All keys are in one tile: delta is the sum of P * dP, without the rounding
-  // of `out`, which would be most of dS's error where keys are few.
-  const bool one_tile = kFew && nk <= W;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
@@ -169,7 +180,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
                  x2_more = x1_more + S::kOwnMore,
                  y1_more = x2_more + S::kOwnMore,
                  y2_more = y1_more + S::kStages * S::kTileMore;
-  const uint32_t bar0 = tc::smem_address(bars);
+  const uint32_t bar0 = tc::smem_address(shared.bars);
   const int steps = (a.dim + 15) / 16;
   const unsigned char* mask = a.mask ? a.mask + k0 : nullptr;
   bool ok = true;
@@ -274,7 +285,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
 
   if (nt > 0) {
     if (warp == kRowWarps) {
-      tc::tmem_alloc(tc::smem_address(&tmem_at), S::kColumns);
+      tc::tmem_alloc(tc::smem_address(&shared.tmem_at), S::kColumns);
     } else if (warp == kRowWarps + 1) {
       if (lane == 0) {
         for (int i = 0; i < kBars; ++i)
@@ -329,7 +340,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         for (int i = 0; i < kEach; ++i) {
           const int at = ((tid >> 7) + i * S::kShare) * 8;
           u[i] = v[i] = make_uint4(0, 0, 0, 0);
-          if (!one_tile && at < a.dim) {
+          if (!kOneTile && at < a.dim) {
             u[i] = *reinterpret_cast<const uint4*>(o + at);
             v[i] = *reinterpret_cast<const uint4*>(d + at);
           }
@@ -360,7 +371,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    tmem = tmem_at;
+    tmem = shared.tmem_at;
   }
 
   if (warp == kRowWarps + 1) {
@@ -416,6 +427,9 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
     const uint32_t mine = tmem + ((uint32_t)group << 21);
     bool open = live;
     float lse2 = -kInf, delta = 0.f;
+    // The scene has one open key, whose P is 1 whatever the scores and its dS
+    // 0 (in the keys' pass: which is the warp's).
+    bool single = false;
     // what the keys' pass needs of this row
     auto put_values = [&](float minus_delta) {
       const uint2 u = three_parts<T>(lse2 / a.scale_log2e, s_exp);
@@ -432,8 +446,11 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
     };
     if constexpr (kKeysPass) {
       open = live && (!mask || __ldg(mask + r));
+      if (__popc(__ballot_sync(kFull, open)) == 1)
+        single = single_key(mask, nk);
     } else if (nt > 0) {
-      if (!one_tile) {
+      single = single_key(mask, nk);
+      if constexpr (!kOneTile) {
 #pragma unroll
         for (int i = 0; i < S::kShare; ++i)
           delta += part_delta[i][group * 32 + lane];
@@ -445,23 +462,9 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
         // a row without keys gets P = 0
         const float x = __ldg(a.lse + row * a.heads + h);
         if (x != -kInf) lse2 = fmaf(x, -kLog2e, (float)p_bits<T>());
-        if (!one_tile && part == 0) put_values(-delta);
+        if (!kOneTile && part == 0) put_values(-delta);
       }
       delta *= -ds_factor;
-    }
-    // A scene's only open key has P = 1 whatever the scores, and dS = 0 (looked
-    // for where all keys are in a tile).
-    bool lone = false;
-    if constexpr (kKeysPass || kFew) {
-      constexpr int kLook = kKeysPass ? kRows : W;
-      if (nk <= kLook) {
-        uint32_t words[kLook / 32];
-        key_words<kLook>(words, mask, 0, nk);
-        int keys = 0;
-#pragma unroll
-        for (int i = 0; i < kLook / 32; ++i) keys += __popc(words[i]);
-        lone = keys == 1;
-      }
     }
     __syncwarp();
     const bool all_open = __all_sync(kFull, open);
@@ -503,7 +506,7 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
           const int first = (begin + t) * W;
           some = mask || first + W > nk;
           if (some) key_words<W>(words, mask, first, nk);
-          if (one_tile) {
+          if constexpr (kOneTile) {
             float sum = 0.f;
             const uint32_t word = some ? my_word(words) : 0xffffffffu;
 #pragma unroll
@@ -565,14 +568,6 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
             }
           }
         }
-        if (lone) {
-#pragma unroll
-          for (int i = 0; i < kMine / 2; ++i) {  // 0, or NaN of what is one
-            float w[2];
-            Vec<T>::unpack2(ds[i], w);
-            ds[i] = pack2<T>(w[0] - w[0], w[1] - w[1]);
-          }
-        }
         // P's and dS's places are free once the last products are complete
         if (t > 0) wait(kOutput, t - 1);
         __syncwarp();
@@ -611,8 +606,9 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
       }
 #pragma unroll
       for (int which = 0; which < (kKeysPass ? 2 : 1); ++which) {
-        const float f = which ? power_of_two(-p_bits<T>())
-                              : a.scale * power_of_two(-bits);
+        const float f = which    ? power_of_two(-p_bits<T>())
+                        : single ? 0.f  // NaN of what is one
+                                 : a.scale * power_of_two(-bits);
         T* out = static_cast<T*>(kKeysPass ? (which ? a.dv : a.dk) : a.dq) + at;
         float* sum =
             a.part + ((kKeysPass ? 2 : 1) * split + which) * parts + at;
@@ -649,6 +645,38 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
       tc::tmem_free(tmem, S::kColumns);
     }
   }
+}
+
+// kShort (queries' pass): scenes of one tile of keys may be among the others.
+// They have code of their own, chosen by the scene, so that a scene's results do
+// not depend on the rest of its batch; in one piece with the other it would cost
+// longer scenes registers (a training step of 8 x 6,000 rows on 1,500 keys 945 us
+// for 920).  It comes first: behind the other it costs 5 rows on 7 keys 22.8 us
+// for 20.8, while a scene of 10 rows on 24,000 keys takes 186.8 us for 182.8
+// without it.
+template <typename T, int kDim, bool kKeysPass, bool kShort>
+__global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
+                                  Shape<kDim, kKeysPass>::kBlocks)
+    cross_backward_kernel(const __grid_constant__ CrossArgs a,
+                          const __grid_constant__ BackMaps maps) {
+  using S = Shape<kDim, kKeysPass>;
+  __shared__ Shared<S, kKeysPass> shared;
+  unsigned unit = blockIdx.x;
+  const int r0 = unit % a.tiles * kRows;
+  unit /= a.tiles;
+  const int split = unit % a.splits;
+  unit /= a.splits;
+  const int hk = unit % a.kv_heads;
+  const int scene = unit / a.kv_heads;
+  const int q0 = __ldg(a.q_seg + scene), k0 = __ldg(a.k_seg + scene);
+  const int n = (__ldg(a.q_seg + scene + 1) - q0) * a.group;  // packed rows
+  const int nk = __ldg(a.k_seg + scene + 1) - k0;
+  if (kShort && nk <= S::kWalk)
+    backward_block<T, kDim, kKeysPass, kShort>(a, maps, shared, q0, n, k0, nk,
+                                               hk, split, r0);
+  else
+    backward_block<T, kDim, kKeysPass, false>(a, maps, shared, q0, n, k0, nk,
+                                              hk, split, r0);
 }
 
 // The parts of a split result added up, four elements a thread.
@@ -703,7 +731,7 @@ Plan backward_plan(const attention_args* a) {
   return p;
 }
 
-template <typename T, int kDim, bool kKeysPass, bool kFew>
+template <typename T, int kDim, bool kKeysPass, bool kShort>
 cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
                         cudaStream_t s) {
   using S = Shape<kDim, kKeysPass>;
@@ -727,12 +755,12 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
                   S::kWalk);
   }
   if (!e)
-    e = cudaFuncSetAttribute(cross_backward_kernel<T, kDim, kKeysPass, kFew>,
+    e = cudaFuncSetAttribute(cross_backward_kernel<T, kDim, kKeysPass, kShort>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              S::kSmem);
   if (e) return e;
   count_launches(1);
-  cross_backward_kernel<T, kDim, kKeysPass, kFew>
+  cross_backward_kernel<T, kDim, kKeysPass, kShort>
       <<<(unsigned)grid, S::kThreads, S::kSmem, s>>>(a, maps);
   if (a.splits > 1) {
     const long long n =
@@ -753,25 +781,14 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
 }
 
 // The queries' pass first: it leaves its rows' lse and delta to the keys'.
-// Scenes of one tile of keys beside others of many take delta from `out` like
-// those: looking for them costs the pass registers (8 scenes of 6000 rows and
-// 1500 keys, both passes: 945 us, without 920), and a batch whose largest has
-// 16 tiles and more has little of its gradients from them.
-template <typename T>
+template <typename T, int kDim>
 cudaError_t launch(const CrossArgs& a, const attention_args* in, const Plan& p,
                    cudaStream_t s) {
-  cudaError_t e;
-  if (a.dim <= 64)
-    e = in->max_k <= 16 * Shape<64, false>::kWalk
-            ? launch_pass<T, 64, false, true>(a, in, p, s)
-            : launch_pass<T, 64, false, false>(a, in, p, s);
-  else
-    e = in->max_k <= 16 * Shape<128, false>::kWalk
-            ? launch_pass<T, 128, false, true>(a, in, p, s)
-            : launch_pass<T, 128, false, false>(a, in, p, s);
-  if (e) return e;
-  return a.dim <= 64 ? launch_pass<T, 64, true, false>(a, in, p, s)
-                     : launch_pass<T, 128, true, false>(a, in, p, s);
+  const bool one_long = a.scenes == 1 && a.n_k > Shape<kDim, false>::kWalk;
+  const cudaError_t e = one_long
+                            ? launch_pass<T, kDim, false, false>(a, in, p, s)
+                            : launch_pass<T, kDim, false, true>(a, in, p, s);
+  return e ? e : launch_pass<T, kDim, true, false>(a, in, p, s);
 }
 
 }  // namespace
@@ -816,6 +833,9 @@ GSA_API int cross_attention_grad(const attention_args* in) {
   a.dk = in->dk;
   a.dv = in->dv;
   cudaStream_t s = (cudaStream_t)in->stream;
-  return type == kF16 ? launch<__half>(a, in, p, s)
-                      : launch<__nv_bfloat16>(a, in, p, s);
+  if (type == kF16)
+    return a.dim <= 64 ? launch<__half, 64>(a, in, p, s)
+                       : launch<__half, 128>(a, in, p, s);
+  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, in, p, s)
+                     : launch<__nv_bfloat16, 128>(a, in, p, s);
 }

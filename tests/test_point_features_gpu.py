@@ -855,3 +855,43 @@ def test_the_error_flag_of_another_stream_is_waited_for():
     assert not side.query()
     with pytest.raises(RuntimeError):
         pairs.check()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (64, FP16), (128, FP16), (128, BF16)])
+@pytest.mark.parametrize("beside", [1100, 1500, 2100])
+@pytest.mark.parametrize("n_k", [1, 2, 5, 64])
+def test_cross_gradients_of_few_keys_do_not_see_longer_scenes(n_k, beside, dim, dtype):
+    # whatever the longest scene of the batch, a short one has the bits that it
+    # has alone, and exactly 0 where its queries have one key
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(340, ([130, 40], [n_k, beside]), 2, 1, dim, dtype)
+    d = normal(341, *q.shape, dtype=dtype)
+
+    def gradients(d, q, k, v, pairs):
+        out, lse = cross_attention(q, k, v, pairs, return_lse=True)
+        return cross_attention_grad(d, q, k, v, out, lse, pairs)
+
+    both = gradients(d, q, k, v, ScenePairs(q_seg, k_seg))
+    alone = gradients(d[:130], q[:130], k[:n_k], v[:n_k], ScenePairs([0, 130], [0, n_k]))
+    for got, want in zip(both, alone):
+        assert torch.equal(got[: len(want)], want)
+    if n_k == 1:
+        assert not both[0][:130].any() and not both[1][:1].any() and both[2][:1].any()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16), (24, FP16)])
+@pytest.mark.parametrize("n_k", [300, 1500, 2100])
+def test_cross_gradients_of_a_single_open_key_among_many(n_k, dim, dtype):
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(345, ([140, 9, 5], [n_k, n_k + 77, 40]), 4, 2, dim, dtype, scale=8.0)
+    mask = torch.zeros(len(k), dtype=torch.bool, device="cuda")
+    mask[[n_k - 1, n_k + 3]] = True
+    mask[k_seg[2]:] = True
+    check_cross(q, k, v, q_seg, k_seg, mask=mask)
+    pairs, d = ScenePairs(q_seg, k_seg), normal(346, *q.shape, dtype=dtype)
+    out, lse = cross_attention(q, k, v, pairs, mask=mask, return_lse=True)
+    dq, dk, dv = cross_attention_grad(d, q, k, v, out, lse, pairs, mask=mask)
+    assert not dq[:149].any() and not dk[: k_seg[2]].any()
+    assert dv[[n_k - 1, n_k + 3]].any() and dq[149:].any() and dk[k_seg[2]:].any()
