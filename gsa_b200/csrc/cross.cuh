@@ -18,7 +18,7 @@ struct CrossArgs {
   float* lse;  // [n_q][heads], natural
   // what the keys' pass needs of a packed row, [kv_heads][n_q * group]: its
   // -lse in units of q k^T (less the factor that P carries) and its -delta, in
-  // three parts of the inputs' type each
+  // four parts of the inputs' type each
   uint4* row_values;
   void *o, *dq, *dk, *dv;
   float* part;      // [splits][rows][heads][dim] partial results
@@ -29,7 +29,6 @@ struct CrossArgs {
       d_head;
   int scenes, heads, kv_heads, group, dim, tiles, splits;
   float scale, scale_log2e;
-  int scale_exponent;  // 1 / scale is at most 2^this, where that is below 2^15
 };
 
 constexpr int kRows = 128;     // rows of a resident tile

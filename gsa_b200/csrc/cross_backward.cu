@@ -24,7 +24,7 @@
 //
 // In the keys' pass lse and delta belong to the columns.  They come from the
 // products themselves: 16 columns more, powers of two on the keys' side and on
-// the walked side -lse / scale and -delta in three parts of the inputs' type
+// the walked side -lse / scale and -delta in four parts of the inputs' type
 // (24 bits and more together), so that S and dP leave the tensor core less lse
 // and delta.  Read from shared memory (131 KB for 128 x 128 scores) they took
 // as long as all the exponentials.
@@ -103,20 +103,29 @@ __device__ __forceinline__ float power_of_two(int e) {  // -126 to 127
   return __int_as_float((127 + e) << 23);
 }
 
-// x as three values of T that stand for multiples of 2^e, 2^(e-8) and
-// 2^(e-19): the exponents keep fp16 from overflowing (x below 2^(e+16), what
-// is beyond gives NaN) and from losing what lies below its normals.
+// x as four values of T that stand for multiples of 2^15, 2^7, 2^-4 and 2^-24:
+// together they hold an x below 2^31 to 24 bits, or to 2^-41, in fp16 too (what
+// is beyond gives NaN there).
 template <typename T>
-__device__ __forceinline__ uint2 three_parts(float x, int e) {
-  float h = to_float(from_float<T>(x * power_of_two(-e))), m = 0.f, l = 0.f;
-  if (fabsf(h) < kInf) {
-    const float r = x - h * power_of_two(e);
-    m = to_float(from_float<T>(r * power_of_two(8 - e)));
-    l = (r - m * power_of_two(e - 8)) * power_of_two(19 - e);
-  } else if (fabsf(x) < kInf) {
-    h = __int_as_float(0x7fffffff);
+__device__ __forceinline__ uint2 four_parts(float x) {
+  constexpr int kExponents[4] = {15, 7, -4, -24};
+  float part[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    part[i] = to_float(from_float<T>(x * power_of_two(-kExponents[i])));
+    if (i == 0 && !(fabsf(part[0]) < kInf)) {
+      if (fabsf(x) < kInf) part[0] = __int_as_float(0x7fffffff);
+      break;
+    }
+    x -= part[i] * power_of_two(kExponents[i]);
   }
-  return make_uint2(pack2<T>(h, m), pack2<T>(l, 0.f));
+  return make_uint2(pack2<T>(part[0], part[1]), pack2<T>(part[2], part[3]));
+}
+// The other side of their product.
+template <typename T>
+__device__ __forceinline__ uint2 four_units() {
+  return make_uint2(pack2<T>(power_of_two(15), power_of_two(7)),
+                    pack2<T>(power_of_two(-4), power_of_two(-24)));
 }
 
 // The last 16 columns of a product by columns, from narrow tiles.
@@ -196,9 +205,6 @@ __device__ __forceinline__ void backward_block(
   };
   const int bits = ds_bits<T>(nk);
   const float ds_factor = power_of_two(bits - p_bits<T>());
-  // the exponents of the further columns' first part: of lse / scale, so that
-  // lse is below 2^16; of delta
-  const int s_exp = a.scale_exponent, d_exp = 8;
 
   // The loading warp: a tile's copies, and what is left to do when they are
   // there.
@@ -313,12 +319,10 @@ __device__ __forceinline__ void backward_block(
         // the resident tiles' further columns, and the second half (zeros) of
         // the walked ones'
         if (tid < kRows) {
+          const uint2 u = four_units<T>();
           for (int x = 0; x < 2; ++x) {
-            const int e = x ? d_exp : s_exp;
             const uint32_t to = x ? x2_more : x1_more;
-            store(to + tc::narrow_offset(tid, 0),
-                  pack2<T>(power_of_two(e), power_of_two(e - 8)),
-                  pack2<T>(power_of_two(e - 19), 0.f));
+            store(to + tc::narrow_offset(tid, 0), u.x, u.y);
             store(to + tc::narrow_offset(tid, 1), 0, 0);
           }
         }
@@ -432,8 +436,8 @@ __device__ __forceinline__ void backward_block(
     bool single = false;
     // what the keys' pass needs of this row
     auto put_values = [&](float minus_delta) {
-      const uint2 u = three_parts<T>(lse2 / a.scale_log2e, s_exp);
-      const uint2 v = three_parts<T>(minus_delta, d_exp);
+      const uint2 u = four_parts<T>(lse2 / a.scale_log2e);
+      const uint2 v = four_parts<T>(minus_delta);
       a.row_values[((long long)hk * a.n_q + q0) * a.group + r] =
           make_uint4(u.x, u.y, v.x, v.y);
     };

@@ -658,8 +658,6 @@ CrossArgs cross_arguments(const attention_args* in) {
   a.dim = (int)in->dim;
   a.scale = (float)in->scale;
   a.scale_log2e = (float)(in->scale * (double)kLog2e);
-  for (double s = in->scale; s < 1. && a.scale_exponent < 15; s *= 2.)
-    ++a.scale_exponent;
   return a;
 }
 

@@ -895,3 +895,25 @@ def test_cross_gradients_of_a_single_open_key_among_many(n_k, dim, dtype):
     dq, dk, dv = cross_attention_grad(d, q, k, v, out, lse, pairs, mask=mask)
     assert not dq[:149].any() and not dk[: k_seg[2]].any()
     assert dv[[n_k - 1, n_k + 3]].any() and dq[149:].any() and dk[k_seg[2]:].any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_cross_fp16_gradients_of_large_scores_and_outputs(dim):
+    # lse of 2^16 and more (320,000 and 2.5 million), and <dout, out> above
+    # 2^24: both enter the keys' pass in parts
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(360, ([9], [2]), 1, 1, dim, FP16)
+    for size, scale in ((200.0, 0.125), (200.0, 1.0), (25.0, 8.0)):
+        q[:], k[:] = size, size
+        check_cross(q, k, v, q_seg, k_seg, scale=scale)
+    q, k, v, q_seg, k_seg = attention_inputs(365, ([9, 4], [2, 50]), 1, 1, dim, FP16)
+    v[:] = v.sign() * 0.5 + 1000.0
+    pairs, d = ScenePairs(q_seg, k_seg), torch.full_like(q, 1000.0)
+    out, lse = cross_attention(q, k, v, pairs, return_lse=True)
+    want = fo.Attention(q, k, v, q_seg, k_seg, dout=d)
+    assert (d.double() * out.double()).sum(-1).min() > 2**24
+    got = cross_attention_grad(d, q, k, v, out, lse, pairs)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        assert t.isfinite().all()
+        want.close(name, t)
