@@ -20,6 +20,10 @@ struct CrossArgs {
   // -lse in units of q k^T (less the factor that P carries) and its -delta, in
   // four parts of the inputs' type each
   uint4* row_values;
+  // fp16 gradients, [scenes][kv_heads][2 + value_chunks]: the bits of the
+  // largest |dout|^2 of a packed row and of the largest |v|^2 of an open key,
+  // and the latter in every `value_rows` keys
+  unsigned* sizes;
   void *o, *dq, *dk, *dv;
   float* part;      // [splits][rows][heads][dim] partial results
   float* part_lse;  // [splits][n_q][heads]
@@ -28,6 +32,7 @@ struct CrossArgs {
   long long q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, d_row,
       d_head;
   int scenes, heads, kv_heads, group, dim, tiles, splits;
+  int value_chunks, value_rows;
   float scale, scale_log2e;
 };
 

@@ -30,8 +30,13 @@
 // as long as all the exponentials.
 //
 // P and dS are rounded to the inputs' type for their products (half a step).
-// For fp16, whose smallest normal is 2^-14, P carries a factor of 2^15 (it is
-// at most 1) and dS one that grows with the number of keys.
+// For fp16, whose normals are 2^-14 to 2^16, P carries a factor of 2^15 (it is
+// at most 1), and dS a power of two that brings its bound, 2 |dout| |v|, to
+// between 2^14 and 2^15: a row's own in the queries' pass, one for a scene and a
+// head of keys in the keys' pass, where rows are summed over.  So nothing
+// overflows, and what is above 2^-28 of the bound keeps all its bits.  A small
+// kernel before the passes finds |v| (8 x 1,500 keys of 8 x 64: 6 us), the
+// queries' pass |dout|.
 //
 // What bounds it, for 128 x 128 scores and a head of 64: 1,400 clocks of
 // products in the keys' pass (1,024 in the queries') beside 1,024 of
@@ -71,7 +76,7 @@ struct Shape {
   static constexpr uint32_t kOut2 = kOut1 + kDim;  // keys' pass: dv
   static constexpr uint32_t kEnd = kKeysPass ? kOut2 + kDim : kOut2;
   static_assert(kEnd <= kColumns, "tensor memory");
-  static_assert(kBlocks * (kSmem + 4096) <= 227 * 1024, "shared memory");
+  static_assert(kBlocks * (kSmem + 5120) <= 227 * 1024, "shared memory");
 };
 
 struct BackMaps {
@@ -89,15 +94,20 @@ enum Bar {
   kBars = 16
 };
 
-// Factors that P and dS carry (2^x).
+// The factor that P carries (2^x).
 template <typename T>
 __device__ __forceinline__ int p_bits() {
   return __is_same(T, __half) ? 15 : 0;
 }
+// An x with |dout| |v| < 2^x, from their squares.
+__device__ __forceinline__ int size_exponent(float d2, float v2) {
+  const int e = ((__float_as_int(d2 * v2) >> 23) & 255) - 127;
+  return (e + 2) >> 1;
+}
+// The factor that dS carries (2^x), |dP| and |delta| being below 2^size.
 template <typename T>
-__device__ __forceinline__ int ds_bits(int keys) {
-  const int b = 31 - __clz(keys | 1) - 10;
-  return __is_same(T, __half) && b > 0 ? b : 0;
+__device__ __forceinline__ int ds_bits(int size) {
+  return __is_same(T, __half) ? 14 - size : 0;
 }
 __device__ __forceinline__ float power_of_two(int e) {  // -126 to 127
   return __int_as_float((127 + e) << 23);
@@ -156,6 +166,7 @@ struct Shared {
   uint64_t bars[kBars];
   uint32_t tmem_at;
   float part_delta[kKeysPass ? 1 : S::kShare][kKeysPass ? 1 : kRows];
+  float part_size[kKeysPass ? 1 : S::kShare][kKeysPass ? 1 : kRows];
 };
 
 // A block's work: rows from r0 on of a scene (n packed rows from q0 on, nk keys
@@ -166,8 +177,8 @@ struct Shared {
 template <typename T, int kDim, bool kKeysPass, bool kOneTile>
 __device__ __forceinline__ void backward_block(
     const CrossArgs& a, const BackMaps& maps,
-    Shared<Shape<kDim, kKeysPass>, kKeysPass>& shared, int q0, int n, int k0,
-    int nk, int hk, int split, int r0) {
+    Shared<Shape<kDim, kKeysPass>, kKeysPass>& shared, int scene, int q0,
+    int n, int k0, int nk, int hk, int split, int r0) {
   using S = Shape<kDim, kKeysPass>;
   constexpr int W = S::kWalk, kRowWarps = S::kRowWarps;
   extern __shared__ uint8_t smem_raw[];
@@ -203,8 +214,10 @@ __device__ __forceinline__ void backward_block(
                  "r"(u1), "r"(0)
                  : "memory");
   };
-  const int bits = ds_bits<T>(nk);
-  const float ds_factor = power_of_two(bits - p_bits<T>());
+  constexpr bool kSizes = __is_same(T, __half);
+  unsigned* sizes =
+      a.sizes + ((long long)scene * a.kv_heads + hk) * (2 + a.value_chunks);
+  unsigned v_size = 0;  // queries' pass: of all keys, known to row warps
 
   // The loading warp: a tile's copies, and what is left to do when they are
   // there.
@@ -344,10 +357,10 @@ __device__ __forceinline__ void backward_block(
         for (int i = 0; i < kEach; ++i) {
           const int at = ((tid >> 7) + i * S::kShare) * 8;
           u[i] = v[i] = make_uint4(0, 0, 0, 0);
-          if (!kOneTile && at < a.dim) {
+          if (!kOneTile && at < a.dim)
             u[i] = *reinterpret_cast<const uint4*>(o + at);
+          if ((!kOneTile || kSizes) && at < a.dim)
             v[i] = *reinterpret_cast<const uint4*>(d + at);
-          }
         }
         const long long head = (long long)hk * a.group;
         load_packed<T, kRows>(
@@ -357,16 +370,26 @@ __device__ __forceinline__ void backward_block(
             c, x2,
             static_cast<const T*>(a.dout) + q0 * a.d_row + head * a.d_head,
             a.d_row, a.d_head, a.group, r0, n);
-        float sum = 0.f;
+        float sum = 0.f, square = 0.f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
           float x[8], y[8];
           Vec<T>::unpack(u[i], x);
           Vec<T>::unpack(v[i], y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
+          for (int e = 0; e < 8; ++e) {
+            sum = fmaf(x[e], y[e], sum);
+            if constexpr (kSizes) square = fmaf(y[e], y[e], square);
+          }
         }
         part_delta[tid >> 7][tid & (kRows - 1)] = sum;
+        if constexpr (kSizes)
+          shared.part_size[tid >> 7][tid & (kRows - 1)] = square;
+      }
+      if constexpr (kSizes && !kKeysPass) {
+        for (int i = lane; i < a.value_chunks; i += 32)
+          v_size = max(v_size, __ldg(sizes + 2 + i));
+        v_size = __reduce_max_sync(kFull, v_size);
       }
       tc::copy_commit();
       tc::copy_wait<0>();
@@ -431,6 +454,7 @@ __device__ __forceinline__ void backward_block(
     const uint32_t mine = tmem + ((uint32_t)group << 21);
     bool open = live;
     float lse2 = -kInf, delta = 0.f;
+    int bits = 0;  // the factor that dS carries
     // The scene has one open key, whose P is 1 whatever the scores and its dS
     // 0 (in the keys' pass: which is the warp's).
     bool single = false;
@@ -452,6 +476,9 @@ __device__ __forceinline__ void backward_block(
       open = live && (!mask || __ldg(mask + r));
       if (__popc(__ballot_sync(kFull, open)) == 1)
         single = single_key(mask, nk);
+      if constexpr (kSizes)
+        bits = ds_bits<T>(size_exponent(__uint_as_float(__ldg(sizes)),
+                                        __uint_as_float(__ldg(sizes + 1))));
     } else if (nt > 0) {
       single = single_key(mask, nk);
       if constexpr (!kOneTile) {
@@ -468,8 +495,24 @@ __device__ __forceinline__ void backward_block(
         if (x != -kInf) lse2 = fmaf(x, -kLog2e, (float)p_bits<T>());
         if (!kOneTile && part == 0) put_values(-delta);
       }
-      delta *= -ds_factor;
+      if constexpr (kSizes) {
+        float size = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::kShare; ++i)
+          size += shared.part_size[i][group * 32 + lane];
+        bits = ds_bits<T>(size_exponent(size, __uint_as_float(v_size)));
+        if (part == 0) {
+          const unsigned most = __reduce_max_sync(
+              kFull, live && size < kInf ? __float_as_uint(size) : 0u);
+          if (lane == 0) {
+            if (most) atomicMax(sizes, most);
+            if (r0 == 0 && group == 0) sizes[1] = v_size;
+          }
+        }
+      }
+      delta *= -power_of_two(bits - p_bits<T>());
     }
+    const float ds_factor = power_of_two(bits - p_bits<T>());
     __syncwarp();
     const bool all_open = __all_sync(kFull, open);
     const uint64_t scale2 = tc::pair(a.scale_log2e, a.scale_log2e);
@@ -676,11 +719,58 @@ __global__ void __launch_bounds__(Shape<kDim, kKeysPass>::kThreads,
   const int n = (__ldg(a.q_seg + scene + 1) - q0) * a.group;  // packed rows
   const int nk = __ldg(a.k_seg + scene + 1) - k0;
   if (kShort && nk <= S::kWalk)
-    backward_block<T, kDim, kKeysPass, kShort>(a, maps, shared, q0, n, k0, nk,
-                                               hk, split, r0);
+    backward_block<T, kDim, kKeysPass, kShort>(a, maps, shared, scene, q0, n, k0,
+                                               nk, hk, split, r0);
   else
-    backward_block<T, kDim, kKeysPass, false>(a, maps, shared, q0, n, k0, nk,
-                                              hk, split, r0);
+    backward_block<T, kDim, kKeysPass, false>(a, maps, shared, scene, q0, n, k0,
+                                              nk, hk, split, r0);
+}
+
+// The largest |v|^2 among the open keys of a chunk, and no |dout|^2 yet.  Maxima
+// of bits, whose order is that of the values; what is not finite is left out (it
+// makes the results that it reaches NaN whatever the factors).
+template <typename T, int kDim>
+__global__ void __launch_bounds__(256)
+    cross_sizes_kernel(const __grid_constant__ CrossArgs a) {
+  constexpr int L = kDim / 8;  // lanes of a row
+  __shared__ unsigned tops[8];
+  const int hk = blockIdx.y, scene = blockIdx.z;
+  const int k0 = __ldg(a.k_seg + scene);
+  const int nk = __ldg(a.k_seg + scene + 1) - k0;
+  const int first = blockIdx.x * a.value_rows;
+  const int rows = min(a.value_rows, nk - first);  // may be negative
+  const int chunk = threadIdx.x % L * 8;
+  const T* v = static_cast<const T*>(a.v) + ((long long)k0 + first) * a.v_row +
+               hk * a.v_head + chunk;
+  const unsigned char* mask = a.mask ? a.mask + k0 + first : nullptr;
+  float most = 0.f;
+#pragma unroll 4
+  for (int i0 = 0; i0 < rows; i0 += 256 / L) {
+    const int i = i0 + threadIdx.x / L;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (i < rows && chunk < a.dim && (!mask || __ldg(mask + i)))
+      u = __ldg(reinterpret_cast<const uint4*>(v + i * a.v_row));
+    float x[8], sum = 0.f;
+    Vec<T>::unpack(u, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    if (sum < kInf) most = fmaxf(most, sum);
+  }
+  const unsigned top = __reduce_max_sync(kFull, __float_as_uint(most));
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const unsigned all = __reduce_max_sync(
+        kFull, threadIdx.x < 8 ? tops[threadIdx.x] : 0u);
+    unsigned* sizes =
+        a.sizes + ((long long)scene * a.kv_heads + hk) * (2 + a.value_chunks);
+    if (threadIdx.x == 0) {
+      sizes[2 + blockIdx.x] = all;
+      if (blockIdx.x == 0) sizes[0] = 0;
+    }
+  }
 }
 
 // The parts of a split result added up, four elements a thread.
@@ -705,7 +795,9 @@ __global__ void __launch_bounds__(256)
 struct Plan {
   long long tiles[2], blocks[2];  // of the keys' pass, of the queries'
   int splits[2];
-  long long values, part;  // bytes
+  long long value_rows, value_chunks;
+  long long values, sizes, part;  // bytes
+  long long all() const { return values + sizes + part; }
 };
 
 Plan backward_plan(const attention_args* a) {
@@ -725,6 +817,14 @@ Plan backward_plan(const attention_args* a) {
     p.blocks[i] *= p.splits[i];
   }
   p.values = 16 * a->n_q * a->heads;
+  p.value_rows = p.value_chunks = p.sizes = 0;
+  if (a->type == kF16 && a->max_k) {
+    // at most 128 chunks, which a warp reads at once
+    p.value_rows = ceil_div(a->max_k, 128) < 64 ? 64 : ceil_div(a->max_k, 128);
+    p.value_chunks = ceil_div(a->max_k, p.value_rows);
+    p.sizes =
+        ceil_div(a->scenes * a->kv_heads * (2 + p.value_chunks), 4) * 16;
+  }
   // the two passes' parts follow one another in the same place
   const long long keys =
       p.splits[0] == 1 ? 0
@@ -788,6 +888,11 @@ cudaError_t launch_pass(CrossArgs a, const attention_args* in, const Plan& p,
 template <typename T, int kDim>
 cudaError_t launch(const CrossArgs& a, const attention_args* in, const Plan& p,
                    cudaStream_t s) {
+  if (__is_same(T, __half) && p.sizes) {
+    count_launches(1);
+    cross_sizes_kernel<T, kDim>
+        <<<dim3(a.value_chunks, a.kv_heads, a.scenes), 256, 0, s>>>(a);
+  }
   const bool one_long = a.scenes == 1 && a.n_k > Shape<kDim, false>::kWalk;
   const cudaError_t e = one_long
                             ? launch_pass<T, kDim, false, false>(a, in, p, s)
@@ -804,7 +909,7 @@ using namespace gsa;
 GSA_API int64_t cross_attention_grad_workspace(const attention_args* in) {
   if (!cross_sizes(in)) return -2;
   const Plan p = backward_plan(in);
-  return p.values + p.part;
+  return p.all();
 }
 
 // See include/point_features.h.
@@ -822,17 +927,20 @@ GSA_API int cross_attention_grad(const attention_args* in) {
     return -2;
   const Plan p = backward_plan(in);
   if (p.blocks[0] > kMaxInt || p.blocks[1] > kMaxInt) return -2;
-  if (p.values + p.part && (!vector_address(in->workspace) ||
-                           in->workspace_bytes < p.values + p.part))
+  if (p.all() && (!vector_address(in->workspace) ||
+                  in->workspace_bytes < p.all()))
     return -2;
   CrossArgs a = cross_arguments(in);
   a.out = in->out.data;
   a.dout = in->dout.data;
   a.d_row = in->dout.row;
   a.d_head = in->dout.head;
-  a.row_values = static_cast<uint4*>(in->workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(in->workspace) +
-                                    p.values);
+  char* at = static_cast<char*>(in->workspace);
+  a.row_values = reinterpret_cast<uint4*>(at);
+  a.sizes = reinterpret_cast<unsigned*>(at + p.values);
+  a.value_rows = (int)p.value_rows;
+  a.value_chunks = (int)p.value_chunks;
+  a.part = reinterpret_cast<float*>(at + p.all() - p.part);
   a.dq = in->dq;
   a.dk = in->dk;
   a.dv = in->dv;

@@ -917,3 +917,58 @@ def test_cross_fp16_gradients_of_large_scores_and_outputs(dim):
     for name, t in zip(("dq", "dk", "dv"), got):
         assert t.isfinite().all()
         want.close(name, t)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lengths", [([130, 9], [64, 5]), ([200, 300], [1500, 90]), ([64, 3], [20000, 4])], ids=str)
+def test_cross_fp16_gradients_grow_with_dout(lengths, dim):
+    # The gradients are linear in dout, and a power of two of it is exact, so
+    # the bounds of their errors grow with it too, but for a result's own step
+    # below fp16's normals (half of it 2^-25).  dS at 2^-13 of its usual size
+    # loses half its bits, and at 2^12 of it overflows, if it is not brought
+    # into fp16's range.
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(350, lengths, 2, 1, dim, FP16, scale=0.125)
+    pairs = ScenePairs(q_seg, k_seg)
+    d = (normal(351, *q.shape).clamp(-3.9, 3.9) * 8).round() / 8  # six bits each
+    d = d.to(FP16)
+    out, lse = cross_attention(q, k, v, pairs, scale=1.0, return_lse=True)
+    one = cross_attention_grad(d, q, k, v, out, lse, pairs, scale=1.0)
+    want = fo.Attention(q, k, v, q_seg, k_seg, scale=1.0, dout=d)
+    for name, t in zip(("dq", "dk", "dv"), one):
+        want.close(name, t)
+    for factor in (2.0**-13, 2.0**-7, 2.0**8, 2.0**12):
+        got = cross_attention_grad(d * factor, q, k, v, out, lse, pairs, scale=1.0)
+        for name, first, t in zip(("dq", "dk", "dv"), one, got):
+            exact, t = getattr(want, name), t.double().cpu()
+            fits = exact.abs() * factor < 65000
+            assert fits.double().mean() > 0.9
+            error = (t - exact * factor).abs()[fits]
+            assert (error <= (getattr(want, name + "_off") * factor)[fits] + 2.0**-25).all(), (name, factor)
+            # and the errors together grow no faster than dout
+            most = 1.5 * factor * (first.double().cpu() - exact).norm() + 2.0**-25 * exact.numel() ** 0.5
+            assert error.norm() <= most, (name, factor, float(error.norm() / most))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_cross_fp16_gradients_of_large_products(dim):
+    # two keys among 24,000 share the weight, and dout v is 10,000 and -10,000:
+    # dS is 5,000 for results of some hundreds
+    q, k, v, q_seg, k_seg = attention_inputs(355, ([3], [24000]), 1, 1, dim, FP16)
+    q[:] = 1.0
+    k[5], k[20001] = 40.0, 40.0
+    k[5, 0, 0], k[5, 0, 1], k[20001, 0, 0], k[20001, 0, 1] = 41.0, 39.0, 39.0, 41.0
+    v[5], v[20001] = 1.0, -1.0
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    pairs = ScenePairs(q_seg, k_seg)
+    for size in (10000.0 / dim, 60000.0):
+        d = torch.full_like(q, size)
+        out, lse = cross_attention(q, k, v, pairs, scale=2.0**-6, return_lse=True)
+        want = fo.Attention(q, k, v, q_seg, k_seg, scale=2.0**-6, dout=d)
+        for name, t in zip(("dq", "dk", "dv"), cross_attention_grad(d, q, k, v, out, lse, pairs, scale=2.0**-6)):
+            exact, t = getattr(want, name), t.double().cpu()
+            fits = exact.abs() < 65504  # three rows of 30,000 in dk and dv, for one: beyond fp16
+            want.close(name, torch.where(fits, t, exact))
+            assert torch.equal(t[~fits], exact[~fits].sign() * math.inf)
