@@ -125,8 +125,9 @@ __device__ __forceinline__ void share(int n, int splits, int which, int* begin,
   *end = *begin + each + (which < rest ? 1 : 0);
 }
 
-// 2^x of a pair without the exponential unit, to 2^-23: n = round(x), then a
-// polynomial of degree 5 in x - n (a Remez fit of 2^f on [-1/2, 1/2]).
+// 2^x of a pair without the exponential unit, to 2^-22 (2.2e-7 at most, of them
+// 1.6e-7 the fit's): n = round(x), then a polynomial of degree 5 in x - n (a Remez
+// fit of 2^f on [-1/2, 1/2]).
 // x = -inf gives exactly 0; x is not NaN and below 128.
 __device__ __forceinline__ void exp2_polynomial(uint64_t x, float* lo,
                                                 float* hi) {

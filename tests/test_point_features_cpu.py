@@ -335,3 +335,19 @@ def test_written_tensors_that_autograd_follows_are_refused():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_exponential_polynomial_is_as_near_as_it_says():
+    text = (ROOT / "gsa_b200" / "csrc" / "cross.cuh").read_text()
+    body = text[text.index("void exp2_polynomial"):]
+    body = body[: body.index("\n}")]
+    stated = re.search(r"without the exponential unit, to 2\^(-\d+)", text).group(1)
+    # the Horner steps in their order, each coefficient given twice
+    numbers = [float(v) for v in re.findall(r"(\d\.?\d*(?:e-?\d+)?)f", body[body.index("uint64_t p ="):])]
+    coefficients = numbers[0::2]
+    assert numbers[1::2] == coefficients and len(coefficients) == 6
+    x = torch.linspace(-0.5, 0.5, 1_000_001, dtype=torch.float64).float().double()
+    p = torch.zeros_like(x)
+    for c in coefficients:  # fused: one rounding to 32 bits a step
+        p = (p * x + torch.tensor(c, dtype=torch.float32).double()).float().double()
+    assert (p / torch.exp2(x) - 1).abs().max() < 2.0 ** int(stated)
