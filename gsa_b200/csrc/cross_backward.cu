@@ -256,7 +256,7 @@ __device__ __forceinline__ void backward_block(
     uint32_t open[W / 32];
     const int full = (whole(t, open) ? kTileFull : kTileRaw) + stage;
     if (t >= S::kStages) wait(kTileFree + stage, t / S::kStages - 1);
-    __syncwarp();
+    if (!__all_sync(kFull, ok)) return false;
     if (tc::elect()) {
       tc::barrier_expect(bar(full), 2 * panels * each * 128);
       const int head = kKeysPass ? hk * a.group : hk;
@@ -267,6 +267,7 @@ __device__ __forceinline__ void backward_block(
       }
     }
     __syncwarp();
+    return true;
   };
   auto finish = [&](int t) {
     const int stage = t % S::kStages;
@@ -402,9 +403,25 @@ __device__ __forceinline__ void backward_block(
   }
 
   if (warp == kRowWarps + 1) {
+    int sent = min(nt, S::kStages);
     for (int t = 0; t < nt; ++t) {
-      if (t >= S::kStages) issue(t);
+      if (t >= S::kStages && issue(t)) sent = t + 1;
       finish(t);
+    }
+    // No copy is under way when the block ends, also where a wait ran out.  Rows
+    // to be cleared were waited for.
+    const bool fine = __all_sync(kFull, ok);
+    for (int t = max(sent - S::kStages, 0); t < sent; ++t) {
+      const int stage = t % S::kStages;
+      uint32_t open[W / 32];
+      const bool all = whole(t, open);
+      int round = t / S::kStages;
+      if (!all && !fine) {
+        round = 0;
+        for (int u = stage; u < t; u += S::kStages) round += !whole(u, open);
+      }
+      if (all || !fine)
+        tc::barrier_wait(bar((all ? kTileFull : kTileRaw) + stage), round & 1);
     }
   } else if (warp == kRowWarps) {
     for (int t = 0; t < nt; ++t) {
@@ -428,6 +445,8 @@ __device__ __forceinline__ void backward_block(
       }
       __syncwarp();
     }
+    // nor is a product
+    if (nt > 0) tc::barrier_wait(bar(kScores), (nt - 1) & 1);
   } else if (warp == kRowWarps + 2) {
     for (int t = 0; t < nt; ++t) {
       const int stage = t % S::kStages;
@@ -445,6 +464,7 @@ __device__ __forceinline__ void backward_block(
       }
       __syncwarp();
     }
+    if (nt > 0) tc::barrier_wait(bar(kOutput), (nt - 1) & 1);
   } else {
     constexpr int kMine = W / S::kShare;  // a thread's columns of its row
     const int part = warp >> 2, group = warp & 3;

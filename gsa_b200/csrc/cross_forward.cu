@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint32_t open[kKeys / 32];
     const int full = (whole(t, open) ? kValuesFull : kValuesRaw) + stage;
     if (round > 0) wait(kKeysFree + stage, round - 1);
-    __syncwarp();
+    if (!__all_sync(kFull, ok)) return false;
     if (tc::elect()) {
       tc::barrier_expect(bar(kKeysFull + stage), panels * kKeys * 128);
       for (int p = 0; p < panels; ++p)
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                      bar(kKeysFull + stage), p * 64, hk, at);
     }
     if (round > 0) wait(kValuesFree + stage, round - 1);
-    __syncwarp();
+    if (!__all_sync(kFull, ok)) return false;
     if (tc::elect()) {
       tc::barrier_expect(bar(full), panels * kKeys * 128);
       for (int p = 0; p < panels; ++p)
@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                      bar(full), p * 64, hk, at);
     }
     __syncwarp();
+    return true;
   };
   auto finish = [&](int t) {
     const int stage = t % S::kStages;
@@ -185,9 +186,30 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   if (warp == 5) {
+    int sent = min(nt, S::kStages);
     for (int t = 0; t < nt; ++t) {
-      if (t >= S::kStages) issue(t);
+      if (t >= S::kStages && issue(t)) sent = t + 1;
       finish(t);
+    }
+    // No copy is under way when the block ends, also where a wait ran out (then
+    // a tile's keys may have been the last).  Rows to be cleared were waited for.
+    if (nt > 0) {
+      const bool fine = __all_sync(kFull, ok);
+      tc::barrier_wait(bar(kQueries), 0);
+      for (int t = max(sent - S::kStages, 0); t < sent + !fine; ++t) {
+        const int stage = t % S::kStages;
+        tc::barrier_wait(bar(kKeysFull + stage), t / S::kStages & 1);
+        uint32_t open[kKeys / 32];
+        const bool all = whole(t, open);
+        int round = t / S::kStages;
+        if (!all && !fine) {
+          round = 0;
+          for (int u = stage; u < t; u += S::kStages) round += !whole(u, open);
+        }
+        if (all || !fine)
+          tc::barrier_wait(bar((all ? kValuesFull : kValuesRaw) + stage),
+                           round & 1);
+      }
     }
   } else if (warp == 4) {
     const int steps = (a.dim + 15) / 16;
@@ -233,6 +255,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         scores(t + 1);
       }
     }
+    // nor is a product
+    if (nt > 0) tc::barrier_wait(bar(kOutput), (nt - 1) & 1);
   } else {
     const int r = r0 + tid;
     const int rows = min(each, n - r0);
