@@ -972,3 +972,42 @@ def test_cross_fp16_gradients_of_large_products(dim):
             fits = exact.abs() < 65504  # three rows of 30,000 in dk and dv, for one: beyond fp16
             want.close(name, torch.where(fits, t, exact))
             assert torch.equal(t[~fits], exact[~fits].sign() * math.inf)
+
+
+@pytest.mark.parametrize("dim", [40, 128])
+def test_cross_fp16_sizes_are_found_anew(dim):
+    # a graph replayed on smaller gradients and values, and calls on two
+    # streams: the factors are those of a call of its own
+    from gsa_b200 import ScenePairs, cross_attention, cross_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(370, ([70, 0, 300], [700, 40, 9000]), 4, 2, dim, FP16)
+    mask = torch.rand(len(k), generator=torch.Generator().manual_seed(371)) < 0.7
+    k[~mask], v[~mask] = math.nan, torch.finfo(FP16).max  # shut values count for nothing
+    mask, pairs = mask.cuda(), ScenePairs(q_seg, k_seg)
+    d = normal(372, *q.shape, dtype=FP16, scale=3000.0)
+
+    def step():
+        out, lse = cross_attention(q, k, v, pairs, mask=mask, return_lse=True)
+        return cross_attention_grad(d, q, k, v, out, lse, pairs, mask=mask)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for shrink in (1.0, 2.0**-14, 2.0**3):
+        d.mul_(shrink)
+        v[mask] *= 0.5
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+        assert all(t.isfinite().all() and t.any() for t in want)
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for got in results for a, b in zip(got, want))
