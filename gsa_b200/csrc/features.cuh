@@ -77,9 +77,7 @@ struct Vec {
       for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 2 && sizeof(T) != 4) unpack2(w[i], f + 2 * i);
-      }
+      for (int i = 0; i < 4; ++i) unpack2(w[i], f + 2 * i);
     }
   }
   static __device__ __forceinline__ void unpack2(uint32_t w, float* f) {

@@ -51,6 +51,7 @@ __device__ __forceinline__ void angle(const RotaryArgs& a, long long row,
 // 8 warps 586, 2 heads 610, 8 heads 751.
 constexpr int kWarps = 4;
 constexpr int kHeadsAhead = 4;
+constexpr int kMultiprocessors = 148;  // of a B200
 
 // kInterleaved: pairs (2p, 2p + 1); else (p, p + P).
 template <typename T, typename Pos, bool kInterleaved>
@@ -184,7 +185,7 @@ cudaError_t launch(RotaryArgs a, int interleaved, cudaStream_t s) {
     // Too few rows to fill the GPU: the heads on blocks of their own, which
     // take the sines again (375 rows of 8 heads: 3.9 us instead of 6.4).
     a.heads_each = a.heads;
-    if (grid.x < 148) {
+    if (grid.x < kMultiprocessors) {
       a.heads_each = a.heads < 65536 ? 2 : 64;
       grid.y = (unsigned)ceil_div(a.heads, a.heads_each);
     }
