@@ -7,7 +7,8 @@
 //
 // over the entries that name a row of the scene's keys and, in padded rows
 // (the radius query's: ascending IDs, then the first again), do not repeat
-// the first entry.  A row without entries gives 0 and lse = -inf.  Backward,
+// the first entry.  A row without entries gives 0 and lse = -inf, one whose
+// scores are all -inf has no softmax and gives NaN for both.  Backward,
 // with p_j = exp(s_j - lse) and delta = <dout, out>:
 //
 //   ds_j = p_j (<dout, v_j> - delta),   dq = scale sum_j ds_j k_j,
@@ -286,7 +287,9 @@ __global__ void __launch_bounds__(kBlock, kResident)
                               g.h * a.o_head + g.j * Vec<T>::V) = acc.pack();
   }
   if (g.j == 0 && a.lse_out)
-    a.lse_out[g.unit] = g.n ? (m + log2f(l)) * kLn2 : -kInf;
+    a.lse_out[g.unit] = !g.n     ? -kInf
+                        : l == 0.f ? __int_as_float(0x7fffffff)
+                                   : (m + log2f(l)) * kLn2;
 }
 
 // dq, and delta for the keys' pass.  Of few entries the rounding of a 16-bit

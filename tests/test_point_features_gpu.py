@@ -1011,3 +1011,21 @@ def test_cross_fp16_sizes_are_found_anew(dim):
                 results.append(step())
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for got in results for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_neighbor_rows_of_minus_infinity_are_nan(dtype):
+    from gsa_b200 import ScenePairs, neighbor_attention, neighbor_attention_grad
+
+    q, k, v, q_seg, k_seg = attention_inputs(380, ([6], [9]), 2, 1, 16, dtype)
+    q[:], k[:4] = 1.0, 0.0
+    k[:4, 0, 0] = -math.inf
+    ids = torch.tensor([[0, 1, 2], [3, 3, 3], [-1, 9, -1], [5, 6, 7], [1, 5, 1], [0, -1, 0]], dtype=torch.int32).cuda()
+    pairs, d = ScenePairs(q_seg, k_seg), normal(381, *q.shape, dtype=dtype)
+    out, lse = neighbor_attention(q, k, v, ids, pairs, return_lse=True)
+    lost = torch.tensor([True, True, False, False, False, True]).cuda()  # entries, but no softmax
+    assert out[lost].isnan().all() and lse[lost].isnan().all() and out[~lost].isfinite().all()
+    assert (lse[2] == -math.inf).all() and not out[2].any() and lse[3:5].isfinite().all()
+    dq, dk, dv = neighbor_attention_grad(d, q, k, v, ids, out, lse, pairs)
+    assert dq[lost].isnan().all() and not dq[2].any() and dq[3].isfinite().all()
+    assert dv[:4].isnan().all() and dv[4:].isfinite().all()
