@@ -44,7 +44,7 @@
 // softmax, weights and products, of which only the next scores run ahead.  8 x
 // 6,000 queries on 1,500 keys, 8 heads of 64 in bf16: about 330 us of the
 // queries' pass and 350 of the keys', 540 TFLOP/s of the five products that
-// count.
+// count; 4 heads of 128 on 2 take 670 us, in fp16 the two take 707 and 680.
 #include "cross.cuh"
 
 namespace gsa {

@@ -24,9 +24,10 @@
 // tensor memory, at most 97 KB of shared memory each).  Below that lie the
 // exponentials (16 a clock on an SM; a quarter are polynomials in the
 // multiply-add units) up to a head of 128, where the products take as long.
-// 8 x 24,000 queries on 6,000 keys, 4 heads of 128: 2.30 to 2.50 ms (the clock
-// falls with the power limit), 945 to 1,020 TFLOP/s; 8 x 6,000 on 1,500, 8
-// heads of 64: 243 us, 607 TFLOP/s.  Tiles of 64 keys with four blocks on an SM
+// 8 x 24,000 queries on 6,000 keys, 4 heads of 128: 2.46 to 2.50 ms replayed from
+// a graph (2.18 before the clock falls with the power limit), 2.54 ms as a call,
+// 929 TFLOP/s; 8 x 6,000 on 1,500, 8 heads of 64: 242 us replayed, 609 TFLOP/s,
+// and 252 us as a call.  Tiles of 64 keys with four blocks on an SM
 // took 253 to 274 us and 2.7 to 2.8 ms, two threads per row 268 us and 2.68 ms;
 // no polynomials, or a third, 2 to 3 % more.
 //

@@ -27,9 +27,9 @@
 // out among the lanes saves instructions but lengthens the chain from load to
 // result (397 us for 388 forward, 488 for 464 forward and back).
 //
-// 192,000 rows of 32 entries, 8 heads of 32 in bf16: 388 us, 1.08 TB/s of
+// 192,000 rows of 32 entries, 8 heads of 32 in bf16: 391 us, 1.07 TB/s of
 // tensors in device memory (418 MB) and 12 TB/s of gathered heads through L1
-// and L2.  48,000 rows, 4 heads of 32 in FP32, forward and back: 462 us, of them
+// and L2.  48,000 rows, 4 heads of 32 in FP32, forward and back: 467 us, of them
 // about 98 forward, 87 for the order of the entries, 103 for dq and 173 for dk
 // and dv.
 #include "features.cuh"
@@ -59,7 +59,7 @@ struct NeighborArgs {
 
 constexpr int kBlock = 128;
 // Blocks of an SM (64 registers a thread): the forward pass of 192,000 rows
-// takes 388 us, with 7 (72 registers) 431, with 9 (spills) 476.
+// took 388 us, with 7 (72 registers) 431, with 9 (spills) 476.
 constexpr int kResident = 8;
 // Entries of a group whose loads are in flight (an earlier form of the forward
 // pass: 514 us with 4, 654 with 8, 549 with 2).

@@ -47,8 +47,9 @@ __device__ __forceinline__ void angle(const RotaryArgs& a, long long row,
   *s = sn * a.amplitude * a.sign;
 }
 
-// 4 warps and 4 heads ahead: 558 us of 1.5 M rows of 4 x 64 FP32 (5.65 TB/s);
-// 8 warps 586, 2 heads 610, 8 heads 751.
+// 4 warps and 4 heads ahead: 558 us of 1.5 M rows of 4 x 64 FP32, the best of many
+// replays (8 warps 586, 2 heads 610, 8 heads 751); the median is 594 (5.30 TB/s),
+// and calls one after another take 626 (5.03 TB/s).
 constexpr int kWarps = 4;
 constexpr int kHeadsAhead = 4;
 constexpr int kMultiprocessors = 148;  // of a B200

@@ -164,7 +164,8 @@ class Batch:
         scene after scene, ``B * sizes[s]`` and ``B * sizes[t]`` rows): what
         ``cross_attention`` between the levels takes, and, for s = t,
         ``neighbor_attention`` along the rows ``ball<s>``; ``hit<s>`` are rows
-        of ``pairs(B, s + 1, s)``."""
+        of ``pairs(B, s + 1, s)``.  Uploads its offsets: made once, outside a
+        graph capture, and kept."""
         from .attention import ScenePairs
 
         return ScenePairs.of_lengths([self.sizes[s]] * B, [self.sizes[t]] * B)

@@ -103,8 +103,9 @@ int cross_attention_grad(const attention_args* a);
 int64_t cross_attention_grad_workspace(const attention_args* a);
 
 /* The same over the keys that a query's row names, for float32 too (a row
- * without entries is one without open keys).  An entry outside the scene's keys is absent; with `padded`, so is one behind
- * the first that repeats it.  Other repeats count each time. */
+ * without entries is one without open keys).  An entry outside the scene's keys
+ * is absent; with `padded`, so is one behind the first that repeats it.  Other
+ * repeats count each time. */
 int neighbor_attention(const attention_args* a);
 int neighbor_attention_grad(const attention_args* a);
 int64_t neighbor_attention_grad_workspace(const attention_args* a);
