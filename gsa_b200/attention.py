@@ -249,7 +249,9 @@ def cross_attention_grad(dout, q, k, v, out, lse, pairs, mask=None, scale=None):
     """``(dq, dk, dv)`` from the gradient of ``cross_attention``'s ``out``;
     the other arguments are that call's, with its ``out`` and ``lse``.  The
     sums have a fixed order: the same arguments give the same bits.  The
-    results take no part in autograd.  FP16: a row whose ``|lse| / scale`` or
+    results take no part in autograd.  Weights are taken again from ``lse``,
+    whose 32 bits leave them off by some 2^-22 ``|lse|`` of themselves (FP16:
+    beyond an ``|lse|`` of 2^22 they may overflow).  FP16: a row whose ``|lse| / scale`` or
     ``|<dout, out>|`` is 2^31 or more makes dk and dv of its scene NaN."""
     _no_second(dout, q, k, v, out, lse)
     call = _Call("cross attention gradient", q, k, v, pairs, scale, _HALF)

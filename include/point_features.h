@@ -96,7 +96,9 @@ int cross_attention(const attention_args* a);
 int64_t cross_attention_workspace(const attention_args* a);
 
 /* The gradients of cross_attention's out, from its out and lse: dq [n_q]
- * [heads][dim], dk and dv [n_k][kv_heads][dim], all of them written.  For
+ * [heads][dim], dk and dv [n_k][kv_heads][dim], all of them written.  Weights
+ * are taken again from lse, whose 32 bits leave them off by some 2^-22 |lse| of
+ * themselves (float16: beyond an |lse| of 2^22 they may overflow).  For
  * float16, rows whose |lse| / scale or |<dout, out>| is 2^31 or more make dk and
  * dv of their scene NaN. */
 int cross_attention_grad(const attention_args* a);
